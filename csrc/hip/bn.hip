@@ -253,8 +253,8 @@ extern "C" int dtfa_bn_eval_coeffs(int C, float eps, const float* gamma, const f
 // ----------------------------------------------------------------------------
 // Elementwise passes.  At ~5 TB/s a CU moves one 16-byte vector every other clock, which leaves ~100 VALU
 // lane-operations per vector: written element by element (bf16 unpack, fma, max, convert, 64-bit index
-// division) these kernels were bound by the vector ALU, not by HBM.  Hence: two fp32 per instruction
-// (v_pk_fma_f32 / v_pk_add_f32), ReLU on the packed bf16 result (v_pk_max_i16), and a vector index that is
+// division) these kernels were bound by the vector ALU, not by HBM.  Hence: fp32 in pairs, unpacked from and
+// rounded to one bf16 word, ReLU on the packed bf16 result (v_pk_max_i16), and a vector index that is
 // divided once per thread and then advanced by additions.
 // ----------------------------------------------------------------------------
 #include "ew_pack.h"
@@ -479,7 +479,7 @@ __global__ void col_partials_kernel(const bf16* __restrict__ a, const bf16* __re
   const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
   const int cg = blockIdx.x * TX + tx;
   const int cvec = C >> 3;
-  // sums kept as fp32 pairs (two channels per register pair): the loop body is v_pk_fma_f32 / v_pk_add_f32
+  // sums kept as fp32 pairs (two channels per register pair)
   f32x2 s1p[4], s2p[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) s1p[j] = s2p[j] = f32x2{0.f, 0.f};

@@ -81,8 +81,8 @@ __global__ void bn_relu_maxpool_fwd_kernel(const bf16* __restrict__ y, const flo
 }
 
 // ReLU fast path of the forward pass.  After the ReLU every candidate is a non-negative bf16, and those
-// order like 16-bit integers, so the window is reduced two values per instruction: the affine map with
-// v_pk_fma_f32, one rounding (v_cvt_pk_bf16_f32), ReLU and running maximum with v_pk_max_i16.  The winning tap
+// order like 16-bit integers, so the window is reduced two values per instruction: the affine map on
+// fp32 pairs, one rounding (v_cvt_pk_bf16_f32), ReLU and running maximum with v_pk_max_i16.  The winning tap
 // is found afterwards by walking the stored candidates backwards and keeping the tap wherever the candidate
 // equals the maximum (so the first maximum wins, as in the scalar form).  Taps outside the image hold -1,
 // which neither wins nor equals a maximum.

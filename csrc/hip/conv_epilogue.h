@@ -378,7 +378,7 @@ __device__ __forceinline__ void conv_epilogue(const ConvArgs& p, f32x16 (&acc)[B
     };
     // two bits of a gate byte -> an AND mask over the two bf16 halves of a word
     auto keep2 = [](unsigned bits) -> unsigned { return ((bits & 1u) ? 0xffffu : 0u) | ((bits & 2u) ? 0xffff0000u : 0u); };
-    f32x2 bs1p[4], bs2p[4];   // EPI 3: the sums as fp32 pairs (v_pk_add_f32 / v_pk_fma_f32)
+    f32x2 bs1p[4], bs2p[4];   // EPI 3: the sums as fp32 pairs
 #pragma unroll
     for (int j = 0; j < 4; ++j) bs1p[j] = bs2p[j] = f32x2{0.f, 0.f};
     // Per element the readback is a handful of operations, but a 128 x 128 tile of a short-reduction layer is

@@ -1,5 +1,5 @@
-// Packed bf16 <-> fp32 helpers of the elementwise passes: two fp32 per instruction (v_pk_fma_f32 /
-// v_pk_add_f32), ReLU and sign bits on the packed bf16 result (v_pk_max_i16).
+// Packed bf16 <-> fp32 helpers of the elementwise passes: fp32 in pairs, one rounding per pair
+// (v_cvt_pk_bf16_f32), ReLU and sign bits on the packed bf16 result (v_pk_max_i16).
 #pragma once
 #include "common.h"
 

@@ -132,7 +132,7 @@ __global__ void avgpool_fwd_kernel(const bf16* __restrict__ x, bf16* __restrict_
 }
 
 // Fixed-window form: one output vector per thread, 32-bit index arithmetic, every tap's load requested before
-// the first is consumed, two fp32 sums per instruction (v_pk_add_f32).  Taps are added in the same (ky, kx)
+// the first is consumed, the fp32 sums kept as pairs.  Taps are added in the same (ky, kx)
 // order as the generic kernel, so the results are identical.
 typedef float pool_f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int pool_u32x4 __attribute__((ext_vector_type(4)));
