@@ -52,7 +52,7 @@ def _identity_spec(name, t, trainable):
 
 def model_variables(model: nn.Module) -> List[VarSpec]:
     """Every checkpointed variable of ``model`` with its TensorFlow name."""
-    from ..models.layers import Conv2d, ConvBnAct, Dense
+    from ..models.layers import Conv2d, ConvBnAct, Dense, LayerNorm
 
     out: List[VarSpec] = []
     for mod in model.modules():
@@ -101,6 +101,9 @@ def model_variables(model: nn.Module) -> List[VarSpec]:
 
             out.append(VarSpec(scope + "/kernel", mod.weight, k_to_tf, k_from_tf, mod.weight.requires_grad))
             out.append(VarSpec(scope + "/bias", mod.bias, b_to_tf, b_from_tf, mod.bias.requires_grad))
+        elif isinstance(mod, LayerNorm):
+            out.append(_identity_spec(scope + "/gamma", mod.gamma, mod.gamma.requires_grad))
+            out.append(_identity_spec(scope + "/beta", mod.beta, mod.beta.requires_grad))
     names = [v.name for v in out]
     if len(set(names)) != len(names):
         raise ValueError("duplicate TensorFlow variable names in model")

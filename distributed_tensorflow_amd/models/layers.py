@@ -148,6 +148,22 @@ class Dense(nn.Module):
         return F.dense(x, self.weight, self.bias, relu=self.relu)
 
 
+class LayerNorm(nn.Module):
+    """Layer normalisation over the last axis with a learned scale and offset (``tf.contrib.layers.layer_norm``'s
+    variable names ``<scope>/gamma`` and ``<scope>/beta``); both stay fp32 when the module is cast to bf16."""
+
+    def __init__(self, features, eps=1e-5, tf_scope: Optional[str] = None):
+        super().__init__()
+        self.features, self.eps, self.tf_scope = features, eps, tf_scope
+        self.gamma = nn.Parameter(torch.ones(features))
+        self.beta = nn.Parameter(torch.zeros(features))
+        self.gamma._keep_fp32 = self.beta._keep_fp32 = True
+
+    def forward(self, x):
+        F.param_fence(self)
+        return F.layer_norm(x, self.gamma, self.beta, eps=self.eps)
+
+
 def cast_for_device(module: nn.Module, device, compute_dtype=None) -> nn.Module:
     """Move a model to ``device``; on a GPU the conv/dense weights become bf16
     while batch-norm parameters, biases and running statistics stay fp32."""

@@ -26,6 +26,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import conv as cv
 from . import kernels as K
@@ -1023,6 +1024,44 @@ def global_avg_pool(x):
     if not _use_hip(x):
         return ref.global_avg_pool(x)
     return _GapFn.apply(x)
+
+
+# ----------------------------------------------------------------------------
+# layer normalisation
+# ----------------------------------------------------------------------------
+class _LayerNormFn(Function):
+    @staticmethod
+    def forward(ctx, x, gamma, beta, eps, params):
+        y, mean, rstd = K.layer_norm_fwd(x, gamma, beta, eps, want_stats=True)
+        ctx.params = params
+        ctx.save_for_backward(x, gamma, mean, rstd)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, gamma, mean, rstd = ctx.saved_tensors
+        want_dx, want_dg, want_db = ctx.needs_input_grad[:3]
+        dx, dg, db = K.layer_norm_bwd(dy, x, gamma, mean, rstd, want_dx, want_dg, want_db)
+        pg, pb = ctx.params
+        return dx, _deliver_small(pg, dg), _deliver_small(pb, db), None, None
+
+
+def layer_norm(x, gamma=None, beta=None, eps: float = 1e-5):
+    """Normalise every vector along the last axis of ``x`` to mean 0 and variance 1 (biased, ``eps`` added to it), then
+    scale by ``gamma`` and shift by ``beta`` (vectors, either may be None).  On the GPU ``x`` is bf16, fp16 or fp32 --
+    contiguous or a channel slice of a wider tensor; other layouts are copied first --, ``gamma`` / ``beta`` are fp32, and
+    the result is contiguous in ``x``'s dtype.  Differentiable once in all three."""
+    if not _use_hip(x):
+        if x.dim() < 1 or x.shape[-1] < 1:
+            raise ValueError("layer_norm: the last axis must not be empty, got shape %s" % (tuple(x.shape),))
+        for t, nm in ((gamma, "gamma"), (beta, "beta")):
+            if t is not None and tuple(t.shape) != (x.shape[-1],):
+                raise ValueError("layer_norm: %s must be a vector of %d elements, got %s" % (nm, x.shape[-1], tuple(t.shape)))
+        return ref.layer_norm(x, gamma, beta, eps)
+    if not _needs_grad(x, gamma, beta):
+        return K.layer_norm_fwd(x, gamma, beta, eps)[0]
+    return _LayerNormFn.apply(x, gamma, beta, eps, (gamma, beta))
 
 
 # ----------------------------------------------------------------------------

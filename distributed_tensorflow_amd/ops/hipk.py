@@ -8,6 +8,7 @@ argument raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from typing import Optional
 
@@ -135,6 +136,10 @@ class _Sigs:
     dtfa_act_l2_bwd = [c_void, c_void, c_void, c_float, c_void, c_ll, c_void]
     dtfa_adam = [c_void, c_void, c_void, c_void, c_int, c_void, c_ll, c_void, c_float, c_float, c_float, c_void]
     dtfa_momentum = [c_void, c_void, c_void, c_int, c_void, c_ll, c_void, c_float, c_float, c_int, c_void]
+    dtfa_layer_norm_fwd = [c_void, c_ll, c_void, c_void, c_void, c_void, c_void, c_ll, c_int, c_float, c_int, c_void]
+    dtfa_layer_norm_bwd_parts = [c_ll, c_int, c_int]
+    dtfa_layer_norm_bwd = [c_void, c_ll, c_void, c_ll, c_void, c_void, c_void, c_void, c_void, c_void, c_void, c_ll, c_int,
+                           c_int, c_void]
     dtfa_cast_f32_bf16 = [c_void, c_void, c_ll, c_void]
     dtfa_mask_mul = [c_void, c_void, c_void, c_ll, c_void]
     dtfa_set_hyper = [c_void, c_float, c_float, c_void]
@@ -151,6 +156,15 @@ class _Sigs:
 
 def stream() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+_same_device = contextlib.nullcontext()
+
+
+def device_of(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one: :func:`stream` then names a stream of that device, and
+    launches and allocations land there."""
+    return _same_device if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

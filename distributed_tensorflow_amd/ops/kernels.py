@@ -530,6 +530,99 @@ def gap_bwd(dy, x_shape):
     return dx
 
 
+# ------------------------------------------------------------------ layer norm
+_LN_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # as in layer_norm.hip
+LAYER_NORM_MAX_C = 1 << 30
+
+
+def _ln_rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """``t`` as rows of its last axis and their pitch in elements: contiguous tensors and channel slices
+    ``buf[..., a:b]`` as they are, anything else (transposed, broadcast) as a contiguous copy."""
+    cols = t.shape[-1]
+    if t.is_contiguous():
+        return t, cols
+    if t.stride(-1) == 1:
+        pitch = want = 0
+        for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if size == 1:
+                continue
+            if pitch == 0:
+                pitch = want = stride
+            if stride != want or pitch < cols:
+                break
+            want = stride * size
+        else:
+            return t, pitch or cols
+    return t.contiguous(), cols
+
+
+def _ln_check(x: torch.Tensor, gamma, beta) -> None:
+    if not x.is_cuda:
+        raise ValueError("layer_norm: x must be a GPU tensor")
+    if x.dtype not in _LN_DTYPES:
+        raise ValueError("layer_norm: x must be bfloat16, float16 or float32, got %s" % x.dtype)
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= LAYER_NORM_MAX_C:
+        raise ValueError("layer_norm: the last axis must have 1 .. 2^30 elements, got shape %s" % (tuple(x.shape),))
+    for t, nm in ((gamma, "gamma"), (beta, "beta")):
+        if t is not None:
+            hipk.require(t, F32, "layer_norm: " + nm)
+            if t.dim() != 1 or t.numel() != x.shape[-1] or t.device != x.device:
+                raise ValueError("layer_norm: %s must be a vector of %d elements on %s, got %s on %s"
+                                 % (nm, x.shape[-1], x.device, tuple(t.shape), t.device))
+
+
+def layer_norm_fwd(x: torch.Tensor, gamma: Optional[torch.Tensor], beta: Optional[torch.Tensor], eps: float,
+                   want_stats: bool = False):
+    """``(x - mean) / sqrt(var + eps) * gamma + beta`` over the last axis, in ``x``'s dtype and contiguous.  ``x``: bf16,
+    fp16 or fp32, contiguous or a channel slice.  Returns ``(y, mean, rstd)``, the statistics one fp32 value a row (None
+    unless ``want_stats``)."""
+    _ln_check(x, gamma, beta)
+    cols = x.shape[-1]
+    rows = x.numel() // cols
+    with hipk.device_of(x):
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        mean = rstd = None
+        if want_stats:
+            mean, rstd = torch.empty((2, rows), dtype=F32, device=x.device).unbind(0)
+        if rows:
+            xr, ldx = _ln_rows(x)
+            hipk.check(hipk.lib().dtfa_layer_norm_fwd(xr.data_ptr(), ldx, hipk.ptr(gamma), hipk.ptr(beta), y.data_ptr(),
+                                                      hipk.ptr(mean), hipk.ptr(rstd), rows, cols, float(eps),
+                                                      _LN_DTYPES[x.dtype], hipk.stream()), "layer_norm_fwd")
+    return y, mean, rstd
+
+
+def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, gamma: Optional[torch.Tensor], mean: torch.Tensor,
+                   rstd: torch.Tensor, want_dx: bool = True, want_dgamma: bool = True, want_dbeta: bool = True):
+    """Gradients ``(dx, dgamma, dbeta)`` of :func:`layer_norm_fwd`, None where not wanted.  ``dgamma`` / ``dbeta`` (fp32)
+    are summed in a fixed order."""
+    _ln_check(x, gamma, None)
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+        raise ValueError("layer_norm backward: dy %s %s does not match x %s %s"
+                         % (tuple(dy.shape), dy.dtype, tuple(x.shape), x.dtype))
+    cols = x.shape[-1]
+    rows = x.numel() // cols
+    for t, nm in ((mean, "mean"), (rstd, "rstd")):
+        hipk.require(t, F32, "layer_norm: " + nm)
+        if t.numel() != rows or t.device != x.device:
+            raise ValueError("layer_norm backward: %s must have one value for each of %d rows" % (nm, rows))
+    with hipk.device_of(x):
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
+        fresh = torch.empty if rows else torch.zeros
+        dgamma = fresh(cols, dtype=F32, device=x.device) if want_dgamma else None
+        dbeta = fresh(cols, dtype=F32, device=x.device) if want_dbeta else None
+        if rows:
+            L, dt = hipk.lib(), _LN_DTYPES[x.dtype]
+            (xr, ldx), (gr, ldg) = _ln_rows(x), _ln_rows(dy)
+            part = None
+            if want_dgamma or want_dbeta:
+                part = torch.empty((L.dtfa_layer_norm_bwd_parts(rows, cols, dt), 2, cols), dtype=F32, device=x.device)
+            hipk.check(L.dtfa_layer_norm_bwd(xr.data_ptr(), ldx, gr.data_ptr(), ldg, hipk.ptr(gamma), mean.data_ptr(),
+                                             rstd.data_ptr(), hipk.ptr(dx), hipk.ptr(part), hipk.ptr(dgamma),
+                                             hipk.ptr(dbeta), rows, cols, dt, hipk.stream()), "layer_norm_bwd")
+    return dx, dgamma, dbeta
+
+
 # ------------------------------------------------------------------ loss
 def softmax_xent(logits: torch.Tensor, labels: torch.Tensor, n_classes: int, grad_scale: float, act_l2: float = 0.0,
                  want_grad: bool = True):

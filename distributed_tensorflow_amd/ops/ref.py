@@ -58,6 +58,18 @@ def batch_norm_eval(y, gamma, beta, run_mean, run_var, eps: float):
     return (y.float() * scale + shift).to(y.dtype)
 
 
+def layer_norm(x, gamma=None, beta=None, eps: float = 1e-5):
+    """Over the last axis (biased variance), computed in fp32 (fp64 for fp64 inputs), rounded once."""
+    xf = x if x.dtype == torch.float64 else x.float()
+    centred = xf - xf.mean(-1, keepdim=True)
+    out = centred * torch.rsqrt(centred.square().mean(-1, keepdim=True) + eps)
+    if gamma is not None:
+        out = out * gamma.to(xf.dtype)
+    if beta is not None:
+        out = out + beta.to(xf.dtype)
+    return out.to(x.dtype)
+
+
 def max_pool(x, k: Tuple[int, int], stride: Tuple[int, int], pads: Tuple[int, int, int, int]):
     pt, pb, pl, pr = pads
     xn = x.permute(0, 3, 1, 2)
