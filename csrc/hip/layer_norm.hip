@@ -17,45 +17,7 @@
 // by element.  Rows too long for the registers take the looping kernels at the end of the file.
 //
 // All arithmetic is fp32; outputs are rounded once.
-#include "common.h"
-
-typedef _Float16 f16;
-
-enum { LN_BF16 = 0, LN_F16 = 1, LN_F32 = 2 };
-
-template <typename T>
-struct LnVec {
-  static constexpr int N = 16 / (int)sizeof(T);
-  typedef T V __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
-};
-typedef float ln_f32x4 __attribute__((ext_vector_type(4), aligned(4)));
-
-// VEC consecutive elements from column `col` of a row of C as fp32; zeros behind the end
-template <typename T, int VEC>
-__device__ __forceinline__ void ln_load(const T* __restrict__ row, int col, int C, float (&v)[VEC]) {
-  if (col + VEC <= C) {
-    const typename LnVec<T>::V w = *(const typename LnVec<T>::V*)(row + col);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = (float)w[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = col + j < C ? (float)row[col + j] : 0.f;
-  }
-}
-
-template <typename T, int VEC>
-__device__ __forceinline__ void ln_store(T* __restrict__ row, int col, int C, const float (&v)[VEC]) {
-  if (col + VEC <= C) {
-    typename LnVec<T>::V w;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) w[j] = (T)v[j];
-    *(typename LnVec<T>::V*)(row + col) = w;
-  } else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j)
-      if (col + j < C) row[col + j] = (T)v[j];
-  }
-}
+#include "row_io.h"
 
 // a per-column fp32 vector (gamma / beta), `fill` where there is none
 template <int VEC>
@@ -63,30 +25,8 @@ __device__ __forceinline__ void ln_param(const float* __restrict__ p, int col, i
   if (p == nullptr) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) v[j] = fill;
-  } else if (col + VEC <= C) {
-#pragma unroll
-    for (int j = 0; j < VEC; j += 4) {
-      const ln_f32x4 w = *(const ln_f32x4*)(p + col + j);
-      v[j] = w[0]; v[j + 1] = w[1]; v[j + 2] = w[2]; v[j + 3] = w[3];
-    }
   } else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = col + j < C ? p[col + j] : 0.f;
-  }
-}
-
-template <int VEC>
-__device__ __forceinline__ void ln_store_f32(float* __restrict__ p, int col, int C, const float (&v)[VEC]) {
-  if (col + VEC <= C) {
-#pragma unroll
-    for (int j = 0; j < VEC; j += 4) {
-      const ln_f32x4 w = {v[j], v[j + 1], v[j + 2], v[j + 3]};
-      *(ln_f32x4*)(p + col + j) = w;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j)
-      if (col + j < C) p[col + j] = v[j];
+    row_load<float, VEC>(p, col, C, v);
   }
 }
 
@@ -131,7 +71,7 @@ struct LnFwd {
 
 template <typename T, int TPR, int NV>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(LnFwd p) {
-  constexpr int VEC = LnVec<T>::N;
+  constexpr int VEC = RowVec<T>::N;
   constexpr int BLOCK = TPR < 256 ? 256 : TPR;
   constexpr int RPB = BLOCK / TPR;  // rows side by side in a workgroup
   __shared__ float red[TPR > 64 ? TPR / 64 : 1];
@@ -146,7 +86,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(L
     float v[NV][VEC];
     float s[1] = {0.f};
 #pragma unroll
-    for (int i = 0; i < NV; ++i) ln_load<T, VEC>(xr, (i * TPR + t) * VEC, p.cols, v[i]);
+    for (int i = 0; i < NV; ++i) row_load<T, VEC>(xr, (i * TPR + t) * VEC, p.cols, v[i]);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -175,7 +115,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(L
         ln_param<VEC>(p.beta, col, p.cols, 0.f, b);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[i][j] = v[i][j] * rstd * g[j] + b[j];
-        ln_store<T, VEC>(yr, col, p.cols, v[i]);
+        row_store<T, VEC>(yr, col, p.cols, v[i]);
       }
       if (p.mean != nullptr && t == 0) {
         p.mean[row] = mean;
@@ -201,7 +141,7 @@ struct LnBwd {
 
 template <typename T, int TPR, int NV, bool PARAMS>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(LnBwd p) {
-  constexpr int VEC = LnVec<T>::N;
+  constexpr int VEC = RowVec<T>::N;
   constexpr int BLOCK = TPR < 256 ? 256 : TPR;
   constexpr int RPB = BLOCK / TPR;
   __shared__ float red[TPR > 64 ? 2 * TPR / 64 : 1];
@@ -227,8 +167,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(L
     float xh[NV][VEC], dy[NV][VEC];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      ln_load<T, VEC>(xr, (i * TPR + t) * VEC, p.cols, xh[i]);
-      ln_load<T, VEC>(gr, (i * TPR + t) * VEC, p.cols, dy[i]);
+      row_load<T, VEC>(xr, (i * TPR + t) * VEC, p.cols, xh[i]);
+      row_load<T, VEC>(gr, (i * TPR + t) * VEC, p.cols, dy[i]);
     }
     const float mean = p.mean[at], rstd = p.rstd[at];
     float s[2] = {0.f, 0.f};
@@ -262,7 +202,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(L
           if (col >= p.cols) continue;
 #pragma unroll
           for (int j = 0; j < VEC; ++j) xh[i][j] = rstd * (dy[i][j] * gam[i][j] - m0 - xh[i][j] * m1);
-          ln_store<T, VEC>(dr, col, p.cols, xh[i]);
+          row_store<T, VEC>(dr, col, p.cols, xh[i]);
         }
       }
     }
@@ -306,8 +246,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(L
     for (int i = 0; i < NV; ++i) {
       const int col = (i * TPR + t) * VEC;
       if (col >= p.cols) continue;
-      ln_store_f32<VEC>(pg, col, p.cols, ag[i]);
-      ln_store_f32<VEC>(pb, col, p.cols, ab[i]);
+      row_store<float, VEC>(pg, col, p.cols, ag[i]);
+      row_store<float, VEC>(pb, col, p.cols, ab[i]);
     }
   }
 }
@@ -337,14 +277,14 @@ __global__ __launch_bounds__(1024) void layer_norm_params_kernel(const float* __
 // ---- rows too long for the registers: the row is walked again instead of held (it comes back from the caches) ----
 template <typename T>
 __global__ __launch_bounds__(1024) void layer_norm_fwd_long_kernel(LnFwd p) {
-  constexpr int VEC = LnVec<T>::N;
+  constexpr int VEC = RowVec<T>::N;
   __shared__ float red[16];
   const float n_c = (float)p.cols;  // (divided by, not multiplied with its inverse: the mean of equal values is that value)
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const T* xr = (const T*)p.x + row * p.ldx;
     float v[VEC], s[1] = {0.f};
     for (long long c = threadIdx.x * VEC; c < p.cols; c += 1024 * VEC) {
-      ln_load<T, VEC>(xr, (int)c, p.cols, v);
+      row_load<T, VEC>(xr, (int)c, p.cols, v);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) s[0] += v[j];
     }
@@ -352,7 +292,7 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_long_kernel(LnFwd p) {
     const float mean = s[0] / n_c;
     s[0] = 0.f;
     for (long long c = threadIdx.x * VEC; c < p.cols; c += 1024 * VEC) {
-      ln_load<T, VEC>(xr, (int)c, p.cols, v);
+      row_load<T, VEC>(xr, (int)c, p.cols, v);
 #pragma unroll
       for (int j = 0; j < VEC; ++j)
         if (c + j < p.cols) s[0] += (v[j] - mean) * (v[j] - mean);
@@ -362,12 +302,12 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_long_kernel(LnFwd p) {
     T* yr = (T*)p.y + row * p.cols;
     for (long long c = threadIdx.x * VEC; c < p.cols; c += 1024 * VEC) {
       float g[VEC], b[VEC];
-      ln_load<T, VEC>(xr, (int)c, p.cols, v);
+      row_load<T, VEC>(xr, (int)c, p.cols, v);
       ln_param<VEC>(p.gamma, (int)c, p.cols, 1.f, g);
       ln_param<VEC>(p.beta, (int)c, p.cols, 0.f, b);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) v[j] = (v[j] - mean) * rstd * g[j] + b[j];
-      ln_store<T, VEC>(yr, (int)c, p.cols, v);
+      row_store<T, VEC>(yr, (int)c, p.cols, v);
     }
     if (p.mean != nullptr && threadIdx.x == 0) {
       p.mean[row] = mean;
@@ -378,7 +318,7 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_long_kernel(LnFwd p) {
 
 template <typename T>
 __global__ __launch_bounds__(1024) void layer_norm_dx_long_kernel(LnBwd p) {
-  constexpr int VEC = LnVec<T>::N;
+  constexpr int VEC = RowVec<T>::N;
   __shared__ float red[32];
   const float n_c = (float)p.cols;  // (divided by, not multiplied with its inverse: the mean of equal values is that value)
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
@@ -387,8 +327,8 @@ __global__ __launch_bounds__(1024) void layer_norm_dx_long_kernel(LnBwd p) {
     const float mean = p.mean[row], rstd = p.rstd[row];
     float x[VEC], d[VEC], g[VEC], s[2] = {0.f, 0.f};
     for (long long c = threadIdx.x * VEC; c < p.cols; c += 1024 * VEC) {
-      ln_load<T, VEC>(xr, (int)c, p.cols, x);
-      ln_load<T, VEC>(gr, (int)c, p.cols, d);
+      row_load<T, VEC>(xr, (int)c, p.cols, x);
+      row_load<T, VEC>(gr, (int)c, p.cols, d);
       ln_param<VEC>(p.gamma, (int)c, p.cols, 1.f, g);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
@@ -400,12 +340,12 @@ __global__ __launch_bounds__(1024) void layer_norm_dx_long_kernel(LnBwd p) {
     const float m0 = s[0] / n_c, m1 = s[1] / n_c;
     T* dr = (T*)p.dx + row * p.cols;
     for (long long c = threadIdx.x * VEC; c < p.cols; c += 1024 * VEC) {
-      ln_load<T, VEC>(xr, (int)c, p.cols, x);
-      ln_load<T, VEC>(gr, (int)c, p.cols, d);
+      row_load<T, VEC>(xr, (int)c, p.cols, x);
+      row_load<T, VEC>(gr, (int)c, p.cols, d);
       ln_param<VEC>(p.gamma, (int)c, p.cols, 1.f, g);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) x[j] = rstd * (d[j] * g[j] - m0 - ((x[j] - mean) * rstd) * m1);
-      ln_store<T, VEC>(dr, (int)c, p.cols, x);
+      row_store<T, VEC>(dr, (int)c, p.cols, x);
     }
   }
 }
@@ -413,15 +353,15 @@ __global__ __launch_bounds__(1024) void layer_norm_dx_long_kernel(LnBwd p) {
 // dgamma / dbeta partials of long rows: a thread owns VEC columns, blockIdx.y a share of the rows
 template <typename T>
 __global__ __launch_bounds__(256) void layer_norm_cols_long_kernel(LnBwd p) {
-  constexpr int VEC = LnVec<T>::N;
+  constexpr int VEC = RowVec<T>::N;
   const long long c = ((long long)blockIdx.x * 256 + threadIdx.x) * VEC;
   if (c >= p.cols) return;
   float ag[VEC], ab[VEC], x[VEC], d[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) ag[j] = ab[j] = 0.f;
   for (long long row = blockIdx.y; row < p.rows; row += gridDim.y) {
-    ln_load<T, VEC>((const T*)p.x + row * p.ldx, (int)c, p.cols, x);
-    ln_load<T, VEC>((const T*)p.dy + row * p.lddy, (int)c, p.cols, d);
+    row_load<T, VEC>((const T*)p.x + row * p.ldx, (int)c, p.cols, x);
+    row_load<T, VEC>((const T*)p.dy + row * p.lddy, (int)c, p.cols, d);
     const float mean = p.mean[row], rstd = p.rstd[row];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
@@ -430,14 +370,14 @@ __global__ __launch_bounds__(256) void layer_norm_cols_long_kernel(LnBwd p) {
     }
   }
   float* pg = p.part + (size_t)blockIdx.y * 2 * p.cols;
-  ln_store_f32<VEC>(pg, (int)c, p.cols, ag);
-  ln_store_f32<VEC>(pg + p.cols, (int)c, p.cols, ab);
+  row_store<float, VEC>(pg, (int)c, p.cols, ag);
+  row_store<float, VEC>(pg + p.cols, (int)c, p.cols, ab);
 }
 
 // ---- host ----
 #define LN_MAX_GRID (1 << 20)
 
-static long long ln_vectors(int cols, int dtype) { return dtype == LN_F32 ? (cols + 3LL) / 4 : (cols + 7LL) / 8; }
+static long long ln_vectors(int cols, int dtype) { return dtype == IO_F32 ? (cols + 3LL) / 4 : (cols + 7LL) / 8; }
 
 template <typename T, int TPR, int NV>
 static int ln_fwd_launch(const LnFwd& p, hipStream_t st) {
@@ -472,9 +412,9 @@ extern "C" int dtfa_layer_norm_fwd(const void* x, long long ldx, const float* ga
   if (cols <= 0 || ldx < 0 || (mean == nullptr) != (rstd == nullptr)) return -1;
   const LnFwd p = {x, ldx, gamma, beta, y, mean, rstd, rows, cols, eps};
   const long long nvec = ln_vectors(cols, dtype);
-  if (dtype == LN_BF16) return ln_fwd<bf16>(p, nvec, st);
-  if (dtype == LN_F16) return ln_fwd<f16>(p, nvec, st);
-  if (dtype == LN_F32) return ln_fwd<float>(p, nvec, st);
+  if (dtype == IO_BF16) return ln_fwd<bf16>(p, nvec, st);
+  if (dtype == IO_F16) return ln_fwd<f16>(p, nvec, st);
+  if (dtype == IO_F32) return ln_fwd<float>(p, nvec, st);
   return -2;
 }
 
@@ -538,9 +478,9 @@ extern "C" int dtfa_layer_norm_bwd(const void* x, long long ldx, const void* dy,
   const LnBwd p = {x, ldx, dy, lddy, gamma, mean, rstd, dx, part, rows, cols};
   const long long nvec = ln_vectors(cols, dtype);
   const int parts = dtfa_layer_norm_bwd_parts(rows, cols, dtype);
-  int rc = dtype == LN_BF16 ? ln_bwd<bf16>(p, nvec, parts, st)
-           : dtype == LN_F16 ? ln_bwd<f16>(p, nvec, parts, st)
-           : dtype == LN_F32 ? ln_bwd<float>(p, nvec, parts, st) : -2;
+  int rc = dtype == IO_BF16 ? ln_bwd<bf16>(p, nvec, parts, st)
+           : dtype == IO_F16 ? ln_bwd<f16>(p, nvec, parts, st)
+           : dtype == IO_F32 ? ln_bwd<float>(p, nvec, parts, st) : -2;
   if (rc != 0 || part == nullptr) return rc;
   hipLaunchKernelGGL(layer_norm_params_kernel, dim3((unsigned)((2LL * cols + 31) / 32)), dim3(1024), 0, st, part, parts,
                      cols, dgamma, dbeta);

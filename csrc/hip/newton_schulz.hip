@@ -1,0 +1,528 @@
+// Orthogonalisation of matrices by Newton-Schulz products, and the Muon optimizer step around it (gfx950).
+//
+//   X_0 = G / (|G|_F + eps)                       A_k = X_k X_k^T   (X_k^T X_k where G has more rows than columns)
+//   B_k = b A_k + c A_k A_k                       X_{k+1} = a X_k + B_k X_k   (a X_k + X_k B_k)
+//   (a, b, c) = (3.4445, -4.7750, 2.0315)
+//
+// which takes every singular value s of G / |G| to f(f(...f(s))), f(s) = a s + b s^3 + c s^5: values above ~1e-2 end in
+// 0.68 .. 1.21.  Small singular values grow by a = 3.44 per iteration, and so does a rounding error made next to them:
+// with operands rounded to 16 bits the result is 1e-3 (well conditioned) to 1e-1 (low rank) off, with fp32 operands
+// 1e-6 to 2e-5.  There is no fp32 matrix instruction at more than a sixteenth of the fp16 rate, so the fp32 operands
+// are kept as two fp16 planes, hi + lo (22 bits), and a product is three v_mfma_f32_32x32x16_f16 --
+// hi*hi + hi*lo + lo*hi, the missing lo*lo is below 2^-22 of the sum of magnitudes -- into one fp32 accumulator.  fp16 and
+// not bf16 planes: the iterates are bounded (|f| <= 1.2024 on [0, 1.2024], so |X| <= 1.21, |A| <= 1.45, |B| <= 2.81 in every
+// entry), so a power of two per matrix puts them into fp16's range with 11 bits each instead of 8.
+//
+// Scales: X is held times S = 2^floor(log2(min(sqrt(rows * cols), 2^15))) -- entries of X_0 are at most 1 and of size
+// 1 / sqrt(rows * cols), later ones at most 1.21: nothing overflows 65504 and the lo plane's smallest step, 2^-24, is below
+// 2^-23 of a typical entry --, A and B times 2^14.  Where the norm is not far above eps, |X_0| = |G| / (|G| + eps) is small,
+// and grows by at most a < 4 per iteration: X_k is held times another 2^e_k, e_0 = -ceil(log2 |X_0|) found on the device
+// (with the norm), e_k = max(0, e_0 - 2 k), and A_k and B_k times 2^(2 e_k), so that vanishing gradients keep their bits.
+//
+// A and B are symmetric: only tiles on and below the diagonal are computed, their mirror images are copies.  All
+// matrices of an optimizer step (or of a batch) go through each stage in one launch, from work lists that name (matrix,
+// tile row, tile column), longest first.  The operands live in a workspace whose planes are padded with zeros to whole
+// tiles, so the products need no bounds checks.
+#include "row_io.h"
+
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+
+#define NS_A 3.4445f
+#define NS_B (-4.7750f)
+#define NS_C 2.0315f
+#define NS_GRAM_SCALE 16384.f  // of A and B
+
+// One matrix.  Offsets in elements of the buffer they point into.
+struct NsMat {
+  long long at;    // of the matrix in the input / output / parameter buffers (rows * cols contiguous values)
+  long long x;     // four planes [rp][cp] in the workspace: X hi, X lo, next X hi, next X lo
+  long long a;     // four planes [mp][mp]: A hi, A lo, B hi, B lo
+  long long part;  // first of its `parts` partial sums of squares
+  int rows, cols;
+  int rp, cp, mp;  // padded rows, columns and min(rows, cols)
+  int parts;
+  int chunk;       // elements per partial sum
+  int tall;        // rows > cols
+  float scale;     // S
+  float lr_scale;  // sqrt(max(1, rows / cols))
+};
+
+struct NsArgs {
+  const NsMat* mats;
+  const int4* chunks;  // {matrix, chunk, -, -}
+  const int4* packs;   // {matrix, tile row, tile column, -}: 64 x 64 tiles of the padded matrix
+  const int4* sym;     // {matrix, tile row, tile column <= tile row, tile edge}: tiles of A and B
+  const int4* full;    // {matrix, tile row, tile column, tile edge}: tiles of X
+  int nchunks, npacks, nsym, nfull;
+  int steps;
+  int dtype;           // of `in` (and `out`): IO_*
+  const void* in;      // the matrices, or their gradients
+  void* out;           // orthogonalised matrices (null: parameter update)
+  float* buf;          // momentum (null: none)
+  float* w;            // parameters
+  bf16* w16;           // their bf16 copy, or null
+  const float* hyper;  // {step size, gradient scale}
+  double* part;        // the partial sums, then e_0 of every matrix
+  f16* ws;
+  long long nparts;
+  float eps, mu, wd;
+  int nesterov;
+};
+
+// ---------------------------------------------------------------- norm and first iterate
+// the value to orthogonalise: the gradient, or the momentum update of it.  Evaluated twice (for the norm, then for X_0)
+// from the same stored values and without contraction, so both see the same bits.
+__device__ __forceinline__ float ns_direction(float g, float buf, float mu, int nesterov) {
+#pragma clang fp contract(off)
+  return nesterov ? g + mu * buf : buf;
+}
+__device__ __forceinline__ float ns_momentum(float g, float buf, float mu) {
+#pragma clang fp contract(off)
+  return mu * buf + g;
+}
+
+// Sums of squares in 64 bits (fp32 squares would overflow at 2e19 and vanish at 1e-23), one per chunk of a matrix, and
+// the momentum update on the way.
+template <typename T, bool MOMENTUM>
+__global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs p) {
+  __shared__ double red[4];
+  const int4 job = p.chunks[blockIdx.x];
+  const NsMat m = p.mats[job.x];
+  const long long n = (long long)m.rows * m.cols;
+  const long long lo = (long long)job.y * m.chunk, hi = lo + m.chunk < n ? lo + m.chunk : n;
+  const T* in = (const T*)p.in + m.at;
+  float* buf = MOMENTUM ? p.buf + m.at : nullptr;
+  const float gs = MOMENTUM ? p.hyper[1] : 1.f;
+  double s = 0.0;
+  for (long long i = lo + threadIdx.x * 8; i < hi; i += 256 * 8) {
+    float g[8], b[8];
+    const int left = hi - i < 8 ? (int)(hi - i) : 8;
+    row_load<T, 8>(in + i, 0, left, g);
+    if (MOMENTUM) {
+      row_load<float, 8>(buf + i, 0, left, b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        g[j] *= gs;
+        b[j] = ns_momentum(g[j], b[j], p.mu);
+        g[j] = ns_direction(g[j], b[j], p.mu, p.nesterov);
+      }
+      row_store<float, 8>(buf + i, 0, left, b);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += j < left ? (double)g[j] * (double)g[j] : 0.0;
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) p.part[m.part + job.y] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+__device__ __forceinline__ void ns_split(float v, f16& hi, f16& lo) {
+  hi = (f16)v;
+  lo = (f16)(v - (float)hi);
+}
+
+// X_0 times S as two fp16 planes, zeros in the padding.  A workgroup writes 64 x 64 values.
+template <typename T, bool MOMENTUM>
+__global__ __launch_bounds__(256) void ns_pack_kernel(NsArgs p) {
+  __shared__ double red[4];
+  const int4 job = p.packs[blockIdx.x];
+  const NsMat m = p.mats[job.x];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < m.parts; i += 256) s += p.part[m.part + i];
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3]));
+  int lift = 0;
+  const double size = norm / (norm + (double)p.eps);
+  if (size > 0.0 && size < 1.0) (void)frexp(size, &lift);   // size * 2^-lift in [0.5, 1)
+  lift = lift < 0 ? -lift : 0;
+  if (job.y == 0 && job.z == 0 && threadIdx.x == 0) p.part[p.nparts + job.x] = (double)lift;
+  const double scale = ldexp((double)m.scale / (norm + (double)p.eps), lift);
+  const T* in = (const T*)p.in + m.at;
+  const float* buf = MOMENTUM ? p.buf + m.at : nullptr;
+  const float gs = MOMENTUM ? p.hyper[1] : 1.f;
+  f16* hi = p.ws + m.x;
+  f16* lo = hi + (size_t)m.rp * m.cp;
+  const int col = job.z * 64 + (threadIdx.x & 7) * 8;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int row = job.y * 64 + h * 32 + (threadIdx.x >> 3);
+    float g[8], b[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] = 0.f;
+    if (row < m.rows && col < m.cols) {
+      row_load<T, 8>(in + (size_t)row * m.cols, col, m.cols, g);
+      if (MOMENTUM) {
+        row_load<float, 8>(buf + (size_t)row * m.cols, col, m.cols, b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] = ns_direction(g[j] * gs, b[j], p.mu, p.nesterov);
+      }
+    }
+    f16x8 vh, vl;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      f16 a, c;
+      ns_split((float)((double)g[j] * scale), a, c);
+      vh[j] = a;
+      vl[j] = c;
+    }
+    *(f16x8*)(hi + (size_t)row * m.cp + col) = vh;
+    *(f16x8*)(lo + (size_t)row * m.cp + col) = vl;
+  }
+}
+
+// ---------------------------------------------------------------- products
+#define NS_BK 32
+
+// 16-byte slot of a tile row's logical chunk: rows of 64 bytes (k contiguous) ...
+__device__ __forceinline__ int ns_swz(int row) { return (row >> 2) & 3; }
+// ... and rows of T fp16 (k is the row), as the transposing reads want it: they touch 64 bytes in each of four rows
+template <int T>
+__device__ __forceinline__ int ns_swz_tr(int row) {
+  return T == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
+}
+
+// An operand of a product: two planes [rows][ld], element (i, k) of the operand at row i, column k (KMAJOR false) or at
+// row k, column i (KMAJOR true); `i0` is the tile's first i.
+struct NsOperand {
+  const f16* hi;
+  const f16* lo;
+  int ld;
+  int i0;
+};
+
+// T x T tile of sum_k P(i, k) Q(j, k) on 2 x 2 waves.  The accumulator of a wave holds the TRANSPOSED tile (Q is the
+// matrix instruction's first operand): lane l, element e of acc[u][v] is column j = v * 32 + (e & 3) + 8 (e >> 2) + 4 (l >> 5)
+// of row i = u * 32 + (l & 31), so four consecutive elements are four consecutive columns.
+//
+// k advances by 32; each of the four waves brings one plane of the next k-tiles (P hi, P lo, Q hi, Q lo) into LDS by
+// LDS-DMA, NST - 1 k-tiles ahead, with counted waits and raw barriers.
+template <int T, bool PK, bool QK>
+__device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& Q, int K, char* smem,
+                                           f32x16 (&acc)[T / 64][T / 64]) {
+  constexpr int PLANE = T * NS_BK * 2;        // bytes
+  constexpr int STAGE = 4 * PLANE;
+  constexpr int NST = T == 128 ? 2 : 4;
+  constexpr int LPS = PLANE / 1024;           // LDS-DMA instructions per wave and k-tile
+  constexpr int MT = T / 64;
+  const int lane = threadIdx.x & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wid >> 1, wc = wid & 1;
+
+  // staging: this wave's plane
+  const bool kmajor = wid < 2 ? PK : QK;
+  const f16* plane = wid == 0 ? P.hi : wid == 1 ? P.lo : wid == 2 ? Q.hi : Q.lo;
+  const int ld = wid < 2 ? P.ld : Q.ld, i0 = wid < 2 ? P.i0 : Q.i0;
+  const f16* src;
+  size_t inst, step;  // elements between the rows of two instructions, between two k-tiles
+  if (kmajor) {
+    constexpr int RPI = 1024 / (T * 2);       // k rows per instruction
+    const int r = lane / (64 / RPI), slot = lane % (64 / RPI);
+    src = plane + (size_t)r * ld + i0 + ((slot ^ ns_swz_tr<T>(r)) << 3);
+    // (an instruction covers 4 or 8 rows and the swizzle has period 4: the slot is the same for all of them)
+    inst = (size_t)RPI * ld;
+    step = (size_t)NS_BK * ld;
+  } else {
+    const int r = lane >> 2, slot = lane & 3; // 16 rows per instruction, the swizzle has period 16
+    src = plane + (size_t)(i0 + r) * ld + ((slot ^ ns_swz(r)) << 3);
+    inst = (size_t)16 * ld;
+    step = NS_BK;
+  }
+  auto stage = [&](int buf) {
+    char* dst = smem + buf * STAGE + wid * PLANE;
+#pragma unroll
+    for (int i = 0; i < LPS; ++i) glds16_untracked(src + i * inst, dst + i * 1024);
+    src += step;
+  };
+
+  // fragments
+  const int tr_q = (lane & 15) >> 2;
+  const int tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  const int tr_k = 8 * (lane >> 5) + tr_q;
+  auto frag = [&](const char* plane_lds, bool km, int row0, int ks) -> f16x8 {
+    if (km) {
+      const int col = row0 + tr_col;
+      union { s16x4 h[2]; f16x8 v; } r;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int krow = ks * 16 + tr_k + 4 * q;
+        const char* at = plane_lds + krow * (T * 2) + (((col >> 3) ^ ns_swz_tr<T>(krow)) << 4) + (col & 7) * 2;
+        r.h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)at);
+      }
+      return r.v;
+    }
+    const int row = row0 + (lane & 31);
+    return *(const f16x8*)(plane_lds + row * 64 + (((ks * 2 + (lane >> 5)) ^ ns_swz(row)) << 4));
+  };
+
+#pragma unroll
+  for (int u = 0; u < MT; ++u)
+#pragma unroll
+    for (int v = 0; v < MT; ++v)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[u][v][e] = 0.f;
+
+  const int nk = K / NS_BK;
+#pragma unroll
+  for (int s = 0; s < NST - 1; ++s)
+    if (s < nk) stage(s);
+  int cur = 0;
+  for (int kt = 0; kt < nk; ++kt) {
+    // k-tile kt has arrived (the NST - 2 behind it may be on their way), and every wave has read k-tile kt - 1
+    if (kt + NST - 2 < nk) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * LPS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (kt + NST - 1 < nk) stage(cur == 0 ? NST - 1 : cur - 1);
+    const char* base = smem + cur * STAGE;
+#pragma unroll
+    for (int ks = 0; ks < NS_BK / 16; ++ks) {
+      f16x8 ph[MT], pl[MT], qh[MT], ql[MT];
+#pragma unroll
+      for (int u = 0; u < MT; ++u) {
+        ph[u] = frag(base, PK, wr * (T / 2) + u * 32, ks);
+        pl[u] = frag(base + PLANE, PK, wr * (T / 2) + u * 32, ks);
+        qh[u] = frag(base + 2 * PLANE, QK, wc * (T / 2) + u * 32, ks);
+        ql[u] = frag(base + 3 * PLANE, QK, wc * (T / 2) + u * 32, ks);
+      }
+#pragma unroll
+      for (int u = 0; u < MT; ++u)
+#pragma unroll
+        for (int v = 0; v < MT; ++v) {
+          acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[v], ph[u], acc[u][v], 0, 0, 0);
+          acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[v], ph[u], acc[u][v], 0, 0, 0);
+          acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[v], pl[u], acc[u][v], 0, 0, 0);
+        }
+    }
+    cur = cur == NST - 1 ? 0 : cur + 1;
+  }
+}
+
+// fp32 tile in LDS: 16-byte writes of 8 rows at a time hit every bank once at this pitch
+#define NS_PITCH(T) ((T) + 4)
+#define NS_LDS_BYTES (128 * NS_PITCH(128) * 4)
+static_assert(NS_LDS_BYTES >= 2 * 4 * 128 * NS_BK * 2 && NS_LDS_BYTES >= 4 * 4 * 64 * NS_BK * 2, "stages fit");
+
+// accumulators -> the tile [i][j] in LDS
+template <int T>
+__device__ __forceinline__ void ns_to_lds(const f32x16 (&acc)[T / 64][T / 64], float* tile) {
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const int i0 = (wid >> 1) * (T / 2) + (lane & 31), j0 = (wid & 1) * (T / 2) + 4 * (lane >> 5);
+  __syncthreads();  // every wave is done with the stages
+#pragma unroll
+  for (int u = 0; u < T / 64; ++u)
+#pragma unroll
+    for (int v = 0; v < T / 64; ++v)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *(f32x4*)(tile + (i0 + u * 32) * NS_PITCH(T) + j0 + v * 32 + 2 * e) =
+            f32x4{acc[u][v][e], acc[u][v][e + 1], acc[u][v][e + 2], acc[u][v][e + 3]};
+  __syncthreads();
+}
+
+__device__ __forceinline__ void ns_join(const f16* hi, const f16* lo, float (&v)[8]) {
+  const f16x8 h = *(const f16x8*)hi, l = *(const f16x8*)lo;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = (float)h[j] + (float)l[j];
+}
+__device__ __forceinline__ void ns_put(f16* hi, f16* lo, const float (&v)[8]) {
+  f16x8 h, l;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    f16 a, b;
+    ns_split(v[j], a, b);
+    h[j] = a;
+    l[j] = b;
+  }
+  *(f16x8*)hi = h;
+  *(f16x8*)lo = l;
+}
+
+// e_k of a matrix
+__device__ __forceinline__ int ns_lift(const NsArgs& p, int mat, int k) {
+  const int e = (int)p.part[p.nparts + mat] - 2 * k;
+  return e > 0 ? e : 0;
+}
+
+// Tile of A = X X^T (or X^T X), or with POLY of B = b A + c A A; and its mirror image.
+template <int T, bool POLY>
+__device__ __forceinline__ void ns_symmetric(const NsArgs& p, const NsMat& m, int ti, int tj, int k, int lift, char* smem) {
+  f32x16 acc[T / 64][T / 64];
+  const size_t xs = (size_t)m.rp * m.cp, as = (size_t)m.mp * m.mp;
+  const f16* x = p.ws + m.x + (k & 1 ? 2 * xs : 0);
+  f16* a = p.ws + m.a;
+  const int i0 = ti * T, j0 = tj * T;
+  if (POLY)
+    ns_product<T, false, false>({a, a + as, m.mp, i0}, {a, a + as, m.mp, j0}, m.mp, smem, acc);
+  else if (m.tall)
+    ns_product<T, true, true>({x, x + xs, m.cp, i0}, {x, x + xs, m.cp, j0}, m.rp, smem, acc);
+  else
+    ns_product<T, false, false>({x, x + xs, m.cp, i0}, {x, x + xs, m.cp, j0}, m.cp, smem, acc);
+  float* tile = (float*)smem;
+  ns_to_lds<T>(acc, tile);
+  f16* out = POLY ? a + 2 * as : a;
+  const float f = POLY ? ldexpf(NS_C / NS_GRAM_SCALE, -2 * lift) : NS_GRAM_SCALE / (m.scale * m.scale);
+  // rows of the tile: eight consecutive columns a thread
+  for (int e = threadIdx.x; e < T * T / 8; e += 256) {
+    const int r = e / (T / 8), c = e % (T / 8) * 8;
+    const size_t at = (size_t)(i0 + r) * m.mp + j0 + c;
+    float* t = tile + r * NS_PITCH(T) + c;
+    float v[8];
+    if (POLY) ns_join(a + at, a + as + at, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = POLY ? NS_B * v[j] + f * t[j] : f * t[j];
+    ns_put(out + at, out + as + at, v);
+    if (ti != tj)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t[j] = v[j];
+  }
+  if (ti == tj) return;
+  __syncthreads();
+  // mirror image: consecutive lanes take consecutive columns of the tile in LDS, eight rows each
+  for (int e = threadIdx.x; e < T * T / 8; e += 256) {
+    const int c = e % T, r = e / T * 8;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = tile[(r + j) * NS_PITCH(T) + c];
+    const size_t at = (size_t)(j0 + c) * m.mp + i0 + r;
+    ns_put(out + at, out + as + at, v);
+  }
+}
+
+enum { NS_NEXT = 0, NS_OUT = 1, NS_APPLY = 2 };
+
+// Tile of a X + B X (or a X + X B): the next iterate, the result, or the parameter update with it.
+template <int T, int WHAT, typename O>
+__device__ __forceinline__ void ns_advance(const NsArgs& p, const NsMat& m, int ti, int tj, int k, int lift, int lift_next,
+                                           char* smem) {
+  f32x16 acc[T / 64][T / 64];
+  const size_t xs = (size_t)m.rp * m.cp, as = (size_t)m.mp * m.mp;
+  const f16* x = p.ws + m.x + (k & 1 ? 2 * xs : 0);
+  f16* next = p.ws + m.x + (k & 1 ? 0 : 2 * xs);
+  const f16* b = p.ws + m.a + 2 * as;
+  const int i0 = ti * T, j0 = tj * T;
+  if (m.tall)
+    ns_product<T, false, false>({x, x + xs, m.cp, i0}, {b, b + as, m.mp, j0}, m.cp, smem, acc);
+  else
+    ns_product<T, false, true>({b, b + as, m.mp, i0}, {x, x + xs, m.cp, j0}, m.rp, smem, acc);
+  float* tile = (float*)smem;
+  ns_to_lds<T>(acc, tile);
+  const float lr = WHAT == NS_APPLY ? p.hyper[0] : 0.f;
+  const float keep = 1.f - lr * p.wd, rate = lr * m.lr_scale;
+  // the result leaves without its scale, the next iterate with its own
+  const float fx = ldexpf(NS_A, lift_next - lift), ft = ldexpf(1.f / NS_GRAM_SCALE, lift_next - 3 * lift);
+  const float unscale = ldexpf(1.f / m.scale, -lift_next);
+  for (int e = threadIdx.x; e < T * T / 8; e += 256) {
+    const int r = e / (T / 8), c = e % (T / 8) * 8;
+    const int row = i0 + r, col = j0 + c;
+    if (WHAT != NS_NEXT && (row >= m.rows || col >= m.cols)) continue;
+    const size_t at = (size_t)row * m.cp + col;
+    const float* t = tile + r * NS_PITCH(T) + c;
+    float v[8];
+    ns_join(x + at, x + xs + at, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = fx * v[j] + ft * t[j];
+    if (WHAT == NS_NEXT) {
+      ns_put(next + at, next + xs + at, v);
+      continue;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= unscale;
+    const size_t flat = m.at + (size_t)row * m.cols;
+    if (WHAT == NS_OUT) {
+      row_store<O, 8>((O*)p.out + flat, col, m.cols, v);
+    } else {
+      float w[8];
+      row_load<float, 8>(p.w + flat, col, m.cols, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = w[j] * keep - rate * v[j];
+      row_store<float, 8>(p.w + flat, col, m.cols, w);
+      if (p.w16 != nullptr) row_store<bf16, 8>(p.w16 + flat, col, m.cols, w);
+    }
+  }
+}
+
+template <bool POLY>
+__global__ __launch_bounds__(256, 2) void ns_symmetric_kernel(NsArgs p, int k) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int4 job = p.sym[blockIdx.x];
+  const NsMat m = p.mats[job.x];
+  const int lift = POLY ? ns_lift(p, job.x, k) : 0;
+  if (job.w == 128)
+    ns_symmetric<128, POLY>(p, m, job.y, job.z, k, lift, smem);
+  else
+    ns_symmetric<64, POLY>(p, m, job.y, job.z, k, lift, smem);
+}
+
+template <int WHAT, typename O>
+__global__ __launch_bounds__(256, 2) void ns_advance_kernel(NsArgs p, int k) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int4 job = p.full[blockIdx.x];
+  const NsMat m = p.mats[job.x];
+  const int lift = ns_lift(p, job.x, k), lift_next = ns_lift(p, job.x, k + 1);
+  if (job.w == 128)
+    ns_advance<128, WHAT, O>(p, m, job.y, job.z, k, lift, lift_next, smem);
+  else
+    ns_advance<64, WHAT, O>(p, m, job.y, job.z, k, lift, lift_next, smem);
+}
+
+// ---------------------------------------------------------------- host
+template <void (*KERNEL)(NsArgs, int)>
+static int ns_tiles(int blocks, const NsArgs& a, int k, hipStream_t st) {
+  // the dynamic-LDS limit is a per-device function attribute: remembered per device
+  static bool attr_set[64] = {};
+  int dev = 0;
+  (void)hipGetDevice(&dev);
+  dev = (dev >= 0 && dev < 64) ? dev : 0;
+  if (!attr_set[dev]) {
+    const int rc = (int)hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, NS_LDS_BYTES);
+    if (rc != 0) return rc;
+    attr_set[dev] = true;
+  }
+  hipLaunchKernelGGL(KERNEL, dim3(blocks), dim3(256), NS_LDS_BYTES, st, a, k);
+  return (int)hipGetLastError();
+}
+
+template <typename T>
+static int ns_first(const NsArgs& a, hipStream_t st) {
+  if (a.buf != nullptr) {
+    hipLaunchKernelGGL((ns_norm_kernel<T, true>), dim3(a.nchunks), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((ns_pack_kernel<T, true>), dim3(a.npacks), dim3(256), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((ns_norm_kernel<T, false>), dim3(a.nchunks), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((ns_pack_kernel<T, false>), dim3(a.npacks), dim3(256), 0, st, a);
+  }
+  return (int)hipGetLastError();
+}
+
+// All matrices of the lists: norm (and momentum), first iterate, `steps` iterations, the last of which writes the result
+// or the parameters.
+extern "C" int dtfa_newton_schulz(const NsArgs* args, hipStream_t st) {
+  const NsArgs a = *args;
+  if (a.nchunks <= 0 || a.npacks <= 0 || a.nsym <= 0 || a.nfull <= 0 || a.steps < 1) return -1;
+  if ((a.out == nullptr) == (a.w == nullptr) || (a.w != nullptr && (a.buf == nullptr || a.hyper == nullptr))) return -2;
+  if (a.out == nullptr && a.dtype == IO_F16) return -3;
+  int rc = a.dtype == IO_BF16 ? ns_first<bf16>(a, st) : a.dtype == IO_F16 ? ns_first<f16>(a, st)
+           : a.dtype == IO_F32 ? ns_first<float>(a, st) : -3;
+  for (int k = 0; k < a.steps && rc == 0; ++k) {
+    rc = ns_tiles<ns_symmetric_kernel<false>>(a.nsym, a, k, st);
+    if (rc == 0) rc = ns_tiles<ns_symmetric_kernel<true>>(a.nsym, a, k, st);
+    if (rc != 0) break;
+    if (k + 1 < a.steps)
+      rc = ns_tiles<ns_advance_kernel<NS_NEXT, float>>(a.nfull, a, k, st);
+    else if (a.out == nullptr)
+      rc = ns_tiles<ns_advance_kernel<NS_APPLY, float>>(a.nfull, a, k, st);
+    else if (a.dtype == IO_BF16)
+      rc = ns_tiles<ns_advance_kernel<NS_OUT, bf16>>(a.nfull, a, k, st);
+    else if (a.dtype == IO_F16)
+      rc = ns_tiles<ns_advance_kernel<NS_OUT, f16>>(a.nfull, a, k, st);
+    else
+      rc = ns_tiles<ns_advance_kernel<NS_OUT, float>>(a.nfull, a, k, st);
+  }
+  return rc;
+}

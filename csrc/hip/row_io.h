@@ -1,0 +1,52 @@
+// Rows of bf16, fp16 or fp32 read and written as fp32, 16 bytes per lane at any element alignment (gfx950 loads and
+// stores them unaligned); the vector that crosses the end of a row goes element by element.
+#pragma once
+#include "common.h"
+
+typedef _Float16 f16;
+
+enum { IO_BF16 = 0, IO_F16 = 1, IO_F32 = 2 };  // element types at the C entry points
+
+template <typename T>
+struct RowVec {
+  static constexpr int N = 16 / (int)sizeof(T);
+  typedef T V __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+};
+
+// VEC (a multiple of the 16-byte vector) consecutive elements from column `col` of a row of C as fp32; zeros behind
+// the end
+template <typename T, int VEC>
+__device__ __forceinline__ void row_load(const T* __restrict__ row, int col, int C, float (&v)[VEC]) {
+  constexpr int N = RowVec<T>::N;
+  static_assert(VEC % N == 0, "whole vectors");
+  if (col + VEC <= C) {
+#pragma unroll
+    for (int i = 0; i < VEC; i += N) {
+      const typename RowVec<T>::V w = *(const typename RowVec<T>::V*)(row + col + i);
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[i + j] = (float)w[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = col + j < C ? (float)row[col + j] : 0.f;
+  }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void row_store(T* __restrict__ row, int col, int C, const float (&v)[VEC]) {
+  constexpr int N = RowVec<T>::N;
+  static_assert(VEC % N == 0, "whole vectors");
+  if (col + VEC <= C) {
+#pragma unroll
+    for (int i = 0; i < VEC; i += N) {
+      typename RowVec<T>::V w;
+#pragma unroll
+      for (int j = 0; j < N; ++j) w[j] = (T)v[i + j];
+      *(typename RowVec<T>::V*)(row + col + i) = w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+      if (col + j < C) row[col + j] = (T)v[j];
+  }
+}

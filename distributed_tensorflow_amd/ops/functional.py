@@ -30,6 +30,7 @@ from torch.autograd.function import once_differentiable
 
 from . import conv as cv
 from . import kernels as K
+from . import newton_schulz as ns
 from . import ref
 
 BF16 = torch.bfloat16
@@ -1062,6 +1063,30 @@ def layer_norm(x, gamma=None, beta=None, eps: float = 1e-5):
     if not _needs_grad(x, gamma, beta):
         return K.layer_norm_fwd(x, gamma, beta, eps)[0]
     return _LayerNormFn.apply(x, gamma, beta, eps, (gamma, beta))
+
+
+# ----------------------------------------------------------------------------
+# orthogonalisation
+# ----------------------------------------------------------------------------
+def orthogonalize(x, steps: int = 5):
+    """Every matrix ``x[..., :, :]`` with its singular values taken towards 1 by ``steps`` Newton-Schulz iterations
+    ``X <- 3.4445 X - 4.7750 (X X^T) X + 2.0315 (X X^T)^2 X`` from ``x / (|x| + 1e-7)`` (Frobenius norm): what the Muon optimizer
+    does to an update.  After five, singular values above about 1 % of the norm lie in 0.68 .. 1.21.  bf16, fp16 or fp32 on
+    the GPU, computed as accurately as in fp32 and rounded once; same shape and dtype, contiguous.  The matrices of a batch are
+    independent, each normalised by itself; a zero matrix stays zero, one with an infinity or NaN becomes NaN as a
+    whole.  Not differentiable."""
+    if x.dim() < 2:
+        raise ValueError("orthogonalize: x must have at least two dimensions, got shape %s" % (tuple(x.shape),))
+    if isinstance(steps, bool) or not isinstance(steps, int) or not 1 <= steps <= ns.MAX_STEPS:
+        raise ValueError("orthogonalize: steps must be a whole number from 1 to %d, got %r" % (ns.MAX_STEPS, steps))
+    if not x.dtype.is_floating_point:
+        raise ValueError("orthogonalize: x must be of a floating-point type, got %s" % x.dtype)
+    ns.check_shape(x.shape[-2], x.shape[-1], "orthogonalize")
+    if _needs_grad(x):
+        raise ValueError("orthogonalize is not differentiable: call it under torch.no_grad() or on x.detach()")
+    if not _use_hip(x):
+        return ref.newton_schulz(x, steps)
+    return ns.orthogonalize(x, steps)
 
 
 # ----------------------------------------------------------------------------

@@ -140,6 +140,7 @@ class _Sigs:
     dtfa_layer_norm_bwd_parts = [c_ll, c_int, c_int]
     dtfa_layer_norm_bwd = [c_void, c_ll, c_void, c_ll, c_void, c_void, c_void, c_void, c_void, c_void, c_void, c_ll, c_int,
                            c_int, c_void]
+    dtfa_newton_schulz = [c_void, c_void]
     dtfa_cast_f32_bf16 = [c_void, c_void, c_ll, c_void]
     dtfa_mask_mul = [c_void, c_void, c_void, c_ll, c_void]
     dtfa_set_hyper = [c_void, c_float, c_float, c_void]

@@ -104,6 +104,23 @@ def dense(x, w, bias=None, relu=False):
     return F.relu(y) if relu else y
 
 
+def newton_schulz(x, steps: int = 5):
+    """``x [..., rows, cols]`` orthogonalised by ``steps`` quintic Newton-Schulz iterations, in fp32 (fp64 for fp64 inputs),
+    rounded once.  The norm, one long sum, is taken in fp64."""
+    a, b, c = 3.4445, -4.7750, 2.0315
+    q = x.double()
+    q = q / (q.square().sum((-1, -2), keepdim=True).sqrt() + 1e-7)
+    q = q if x.dtype == torch.float64 else q.float()
+    tall = q.shape[-2] > q.shape[-1]
+    if tall:
+        q = q.transpose(-1, -2)
+    q = q.contiguous()
+    for _ in range(steps):
+        s = q @ q.transpose(-1, -2).contiguous()
+        q = a * q + (b * s + c * (s @ s)) @ q
+    return (q.transpose(-1, -2) if tall else q).to(x.dtype).contiguous()
+
+
 def dropout(x, rate: float, training: bool, generator: Optional[torch.Generator] = None):
     if not training or rate <= 0.0:
         return x
