@@ -48,13 +48,25 @@ struct NsMat {
   float lr_scale;  // sqrt(max(1, rows / cols))
 };
 
+// One workgroup of a product stage: the tile (ti, tj) of `edge` x `edge` values, summed over k0 <= k < k1.  Where the
+// reduction is cut in several jobs, each leaves its fp32 sums in slab `slab` (in units of 64 x 64 values), else -1; the
+// job that joins them (NsArgs::gram_joins) has the first one's number and k0 = how many there are.
+struct NsJob {
+  int mat;  // -1: nothing (the lists are interleaved from eight queues of equal length)
+  int ti, tj, edge;
+  int k0, k1;
+  int slab, pad;
+};
+
 struct NsArgs {
   const NsMat* mats;
-  const int4* chunks;  // {matrix, chunk, -, -}
-  const int4* packs;   // {matrix, tile row, tile column, -}: 64 x 64 tiles of the padded matrix
-  const int4* sym;     // {matrix, tile row, tile column <= tile row, tile edge}: tiles of A and B
-  const int4* full;    // {matrix, tile row, tile column, tile edge}: tiles of X
-  int nchunks, npacks, nsym, nfull;
+  const int4* chunks;       // {matrix, chunk, -, -}
+  const int4* packs;        // {matrix, tile row, tile column, -}: 64 x 64 tiles of the padded matrix
+  const NsJob* gram;        // tiles of A, tj <= ti
+  const NsJob* gram_joins;
+  const NsJob* poly;        // tiles of B, tj <= ti
+  const NsJob* full;        // tiles of X
+  int nchunks, npacks, ngram, njoin, npoly, nfull;
   int steps;
   int dtype;           // of `in` (and `out`): IO_*
   const void* in;      // the matrices, or their gradients
@@ -64,6 +76,7 @@ struct NsArgs {
   bf16* w16;           // their bf16 copy, or null
   const float* hyper;  // {step size, gradient scale}
   double* part;        // the partial sums, then e_0 of every matrix
+  float* slabs;
   f16* ws;
   long long nparts;
   float eps, mu, wd;
@@ -196,14 +209,16 @@ struct NsOperand {
   int i0;
 };
 
-// T x T tile of sum_k P(i, k) Q(j, k) on 2 x 2 waves.  The accumulator of a wave holds the TRANSPOSED tile (Q is the
-// matrix instruction's first operand): lane l, element e of acc[u][v] is column j = v * 32 + (e & 3) + 8 (e >> 2) + 4 (l >> 5)
-// of row i = u * 32 + (l & 31), so four consecutive elements are four consecutive columns.
+// T x T tile of sum_k P(i, k) Q(j, k), k0 <= k < k1, on 2 x 2 waves.  The accumulator of a wave holds the TRANSPOSED tile
+// (Q is the matrix instruction's first operand): lane l, element e of acc[u][v] is column
+// j = v * 32 + (e & 3) + 8 (e >> 2) + 4 (l >> 5) of row i = u * 32 + (l & 31), so four consecutive elements are four
+// consecutive columns.
 //
 // k advances by 32; each of the four waves brings one plane of the next k-tiles (P hi, P lo, Q hi, Q lo) into LDS by
-// LDS-DMA, NST - 1 k-tiles ahead, with counted waits and raw barriers.
+// LDS-DMA, NST - 1 k-tiles ahead, with counted waits and raw barriers; the fragments of the next 16 k are read while the
+// matrix instructions of the present ones run.
 template <int T, bool PK, bool QK>
-__device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& Q, int K, char* smem,
+__device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& Q, int k0, int k1, char* smem,
                                            f32x16 (&acc)[T / 64][T / 64]) {
   constexpr int PLANE = T * NS_BK * 2;        // bytes
   constexpr int STAGE = 4 * PLANE;
@@ -223,13 +238,13 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
   if (kmajor) {
     constexpr int RPI = 1024 / (T * 2);       // k rows per instruction
     const int r = lane / (64 / RPI), slot = lane % (64 / RPI);
-    src = plane + (size_t)r * ld + i0 + ((slot ^ ns_swz_tr<T>(r)) << 3);
+    src = plane + (size_t)(k0 + r) * ld + i0 + ((slot ^ ns_swz_tr<T>(r)) << 3);
     // (an instruction covers 4 or 8 rows and the swizzle has period 4: the slot is the same for all of them)
     inst = (size_t)RPI * ld;
     step = (size_t)NS_BK * ld;
   } else {
     const int r = lane >> 2, slot = lane & 3; // 16 rows per instruction, the swizzle has period 16
-    src = plane + (size_t)(i0 + r) * ld + ((slot ^ ns_swz(r)) << 3);
+    src = plane + (size_t)(i0 + r) * ld + k0 + ((slot ^ ns_swz(r)) << 3);
     inst = (size_t)16 * ld;
     step = NS_BK;
   }
@@ -259,6 +274,37 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
     const int row = row0 + (lane & 31);
     return *(const f16x8*)(plane_lds + row * 64 + (((ks * 2 + (lane >> 5)) ^ ns_swz(row)) << 4));
   };
+  f16x8 ph[2][MT], pl[2][MT], qh[2][MT], ql[2][MT];
+  auto load_frags = [&](int buf, int ks, int to) {
+    const char* base = smem + buf * STAGE;
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+      ph[to][u] = frag(base, PK, wr * (T / 2) + u * 32, ks);
+      qh[to][u] = frag(base + 2 * PLANE, QK, wc * (T / 2) + u * 32, ks);
+    }
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+      ql[to][u] = frag(base + 3 * PLANE, QK, wc * (T / 2) + u * 32, ks);
+      pl[to][u] = frag(base + PLANE, PK, wr * (T / 2) + u * 32, ks);
+    }
+  };
+  auto multiply = [&](int from) {
+#pragma unroll
+    for (int u = 0; u < MT; ++u)
+#pragma unroll
+      for (int v = 0; v < MT; ++v)
+        acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[from][v], ph[from][u], acc[u][v], 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < MT; ++u)
+#pragma unroll
+      for (int v = 0; v < MT; ++v)
+        acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[from][v], ph[from][u], acc[u][v], 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < MT; ++u)
+#pragma unroll
+      for (int v = 0; v < MT; ++v)
+        acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[from][v], pl[from][u], acc[u][v], 0, 0, 0);
+  };
 
 #pragma unroll
   for (int u = 0; u < MT; ++u)
@@ -267,39 +313,37 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[u][v][e] = 0.f;
 
-  const int nk = K / NS_BK;
+  const int nk = (k1 - k0) / NS_BK;
 #pragma unroll
   for (int s = 0; s < NST - 1; ++s)
     if (s < nk) stage(s);
-  int cur = 0;
-  for (int kt = 0; kt < nk; ++kt) {
-    // k-tile kt has arrived (the NST - 2 behind it may be on their way), and every wave has read k-tile kt - 1
+  // waits until k-tile kt has arrived (the NST - 2 behind it may be on their way) and this wave's reads are done; after
+  // the barrier that holds for every wave
+  auto arrive = [&](int kt) {
     if (kt + NST - 2 < nk) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * LPS) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (kt + NST - 1 < nk) stage(cur == 0 ? NST - 1 : cur - 1);
-    const char* base = smem + cur * STAGE;
-#pragma unroll
-    for (int ks = 0; ks < NS_BK / 16; ++ks) {
-      f16x8 ph[MT], pl[MT], qh[MT], ql[MT];
-#pragma unroll
-      for (int u = 0; u < MT; ++u) {
-        ph[u] = frag(base, PK, wr * (T / 2) + u * 32, ks);
-        pl[u] = frag(base + PLANE, PK, wr * (T / 2) + u * 32, ks);
-        qh[u] = frag(base + 2 * PLANE, QK, wc * (T / 2) + u * 32, ks);
-        ql[u] = frag(base + 3 * PLANE, QK, wc * (T / 2) + u * 32, ks);
-      }
-#pragma unroll
-      for (int u = 0; u < MT; ++u)
-#pragma unroll
-        for (int v = 0; v < MT; ++v) {
-          acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[v], ph[u], acc[u][v], 0, 0, 0);
-          acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[v], ph[u], acc[u][v], 0, 0, 0);
-          acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[v], pl[u], acc[u][v], 0, 0, 0);
-        }
+  };
+  arrive(0);
+  if (NST - 1 < nk) stage(NST - 1);
+  load_frags(0, 0, 0);
+  int cur = 0;
+  for (int kt = 0; kt < nk; ++kt) {
+    const int nxt = cur == NST - 1 ? 0 : cur + 1;
+    load_frags(cur, 1, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(0);
+    __builtin_amdgcn_sched_barrier(0);
+    if (kt + 1 < nk) {
+      arrive(kt + 1);  // ... and k-tile kt has been read by every wave: its slot takes k-tile kt + NST
+      if (kt + NST < nk) stage(cur);
+      load_frags(nxt, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    cur = cur == NST - 1 ? 0 : cur + 1;
+    multiply(1);
+    __builtin_amdgcn_sched_barrier(0);
+    cur = nxt;
   }
 }
 
@@ -349,23 +393,13 @@ __device__ __forceinline__ int ns_lift(const NsArgs& p, int mat, int k) {
   return e > 0 ? e : 0;
 }
 
-// Tile of A = X X^T (or X^T X), or with POLY of B = b A + c A A; and its mirror image.
+// The fp32 tile in LDS, sums over all k, becomes the tile of A, or with POLY of B = b A + c A A, and its mirror image.
 template <int T, bool POLY>
-__device__ __forceinline__ void ns_symmetric(const NsArgs& p, const NsMat& m, int ti, int tj, int k, int lift, char* smem) {
-  f32x16 acc[T / 64][T / 64];
-  const size_t xs = (size_t)m.rp * m.cp, as = (size_t)m.mp * m.mp;
-  const f16* x = p.ws + m.x + (k & 1 ? 2 * xs : 0);
+__device__ __forceinline__ void ns_symmetric_out(const NsArgs& p, const NsMat& m, int ti, int tj, int lift, float* tile) {
+  const size_t as = (size_t)m.mp * m.mp;
   f16* a = p.ws + m.a;
-  const int i0 = ti * T, j0 = tj * T;
-  if (POLY)
-    ns_product<T, false, false>({a, a + as, m.mp, i0}, {a, a + as, m.mp, j0}, m.mp, smem, acc);
-  else if (m.tall)
-    ns_product<T, true, true>({x, x + xs, m.cp, i0}, {x, x + xs, m.cp, j0}, m.rp, smem, acc);
-  else
-    ns_product<T, false, false>({x, x + xs, m.cp, i0}, {x, x + xs, m.cp, j0}, m.cp, smem, acc);
-  float* tile = (float*)smem;
-  ns_to_lds<T>(acc, tile);
   f16* out = POLY ? a + 2 * as : a;
+  const int i0 = ti * T, j0 = tj * T;
   const float f = POLY ? ldexpf(NS_C / NS_GRAM_SCALE, -2 * lift) : NS_GRAM_SCALE / (m.scale * m.scale);
   // rows of the tile: eight consecutive columns a thread
   for (int e = threadIdx.x; e < T * T / 8; e += 256) {
@@ -394,22 +428,65 @@ __device__ __forceinline__ void ns_symmetric(const NsArgs& p, const NsMat& m, in
   }
 }
 
+// Tile of A = X X^T (or X^T X) or, with POLY, of A A; with a slab, only the sums over the job's share of k.
+template <int T, bool POLY>
+__device__ __forceinline__ void ns_symmetric(const NsArgs& p, const NsMat& m, const NsJob& job, int k, int lift, char* smem) {
+  f32x16 acc[T / 64][T / 64];
+  const size_t xs = (size_t)m.rp * m.cp, as = (size_t)m.mp * m.mp;
+  const f16* x = p.ws + m.x + (k & 1 ? 2 * xs : 0);
+  const f16* a = p.ws + m.a;
+  const int i0 = job.ti * T, j0 = job.tj * T;
+  if (POLY)
+    ns_product<T, false, false>({a, a + as, m.mp, i0}, {a, a + as, m.mp, j0}, job.k0, job.k1, smem, acc);
+  else if (m.tall)
+    ns_product<T, true, true>({x, x + xs, m.cp, i0}, {x, x + xs, m.cp, j0}, job.k0, job.k1, smem, acc);
+  else
+    ns_product<T, false, false>({x, x + xs, m.cp, i0}, {x, x + xs, m.cp, j0}, job.k0, job.k1, smem, acc);
+  float* tile = (float*)smem;
+  ns_to_lds<T>(acc, tile);
+  if (!POLY && job.slab >= 0) {
+    float* slab = p.slabs + (size_t)job.slab * 4096;
+    for (int e = threadIdx.x; e < T * T / 4; e += 256)
+      *(f32x4*)(slab + e * 4) = *(const f32x4*)(tile + e / (T / 4) * NS_PITCH(T) + e % (T / 4) * 4);
+    return;
+  }
+  ns_symmetric_out<T, POLY>(p, m, job.ti, job.tj, lift, tile);
+}
+
+// Sums of the slabs of a tile, in order.
+template <int T>
+__device__ __forceinline__ void ns_join_slabs(const NsArgs& p, const NsMat& m, const NsJob& job, char* smem) {
+  float* tile = (float*)smem;
+  const float* slab = p.slabs + (size_t)job.slab * 4096;
+  for (int e = threadIdx.x; e < T * T / 4; e += 256) {
+    f32x4 v = *(const f32x4*)(slab + e * 4);
+    for (int i = 1; i < job.k0; ++i) {
+      const f32x4 w = *(const f32x4*)(slab + (size_t)i * T * T + e * 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += w[j];
+    }
+    *(f32x4*)(tile + e / (T / 4) * NS_PITCH(T) + e % (T / 4) * 4) = v;
+  }
+  __syncthreads();
+  ns_symmetric_out<T, false>(p, m, job.ti, job.tj, 0, tile);
+}
+
 enum { NS_NEXT = 0, NS_OUT = 1, NS_APPLY = 2 };
 
 // Tile of a X + B X (or a X + X B): the next iterate, the result, or the parameter update with it.
 template <int T, int WHAT, typename O>
-__device__ __forceinline__ void ns_advance(const NsArgs& p, const NsMat& m, int ti, int tj, int k, int lift, int lift_next,
+__device__ __forceinline__ void ns_advance(const NsArgs& p, const NsMat& m, const NsJob& job, int k, int lift, int lift_next,
                                            char* smem) {
   f32x16 acc[T / 64][T / 64];
   const size_t xs = (size_t)m.rp * m.cp, as = (size_t)m.mp * m.mp;
   const f16* x = p.ws + m.x + (k & 1 ? 2 * xs : 0);
   f16* next = p.ws + m.x + (k & 1 ? 0 : 2 * xs);
   const f16* b = p.ws + m.a + 2 * as;
-  const int i0 = ti * T, j0 = tj * T;
+  const int i0 = job.ti * T, j0 = job.tj * T;
   if (m.tall)
-    ns_product<T, false, false>({x, x + xs, m.cp, i0}, {b, b + as, m.mp, j0}, m.cp, smem, acc);
+    ns_product<T, false, false>({x, x + xs, m.cp, i0}, {b, b + as, m.mp, j0}, job.k0, job.k1, smem, acc);
   else
-    ns_product<T, false, true>({b, b + as, m.mp, i0}, {x, x + xs, m.cp, j0}, m.rp, smem, acc);
+    ns_product<T, false, true>({b, b + as, m.mp, i0}, {x, x + xs, m.cp, j0}, job.k0, job.k1, smem, acc);
   float* tile = (float*)smem;
   ns_to_lds<T>(acc, tile);
   const float lr = WHAT == NS_APPLY ? p.hyper[0] : 0.f;
@@ -450,25 +527,37 @@ __device__ __forceinline__ void ns_advance(const NsArgs& p, const NsMat& m, int 
 template <bool POLY>
 __global__ __launch_bounds__(256, 2) void ns_symmetric_kernel(NsArgs p, int k) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int4 job = p.sym[blockIdx.x];
-  const NsMat m = p.mats[job.x];
-  const int lift = POLY ? ns_lift(p, job.x, k) : 0;
-  if (job.w == 128)
-    ns_symmetric<128, POLY>(p, m, job.y, job.z, k, lift, smem);
+  const NsJob job = (POLY ? p.poly : p.gram)[blockIdx.x];
+  if (job.mat < 0) return;
+  const NsMat m = p.mats[job.mat];
+  const int lift = POLY ? ns_lift(p, job.mat, k) : 0;
+  if (job.edge == 128)
+    ns_symmetric<128, POLY>(p, m, job, k, lift, smem);
   else
-    ns_symmetric<64, POLY>(p, m, job.y, job.z, k, lift, smem);
+    ns_symmetric<64, POLY>(p, m, job, k, lift, smem);
+}
+
+__global__ __launch_bounds__(256, 2) void ns_join_kernel(NsArgs p, int) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const NsJob job = p.gram_joins[blockIdx.x];
+  const NsMat m = p.mats[job.mat];
+  if (job.edge == 128)
+    ns_join_slabs<128>(p, m, job, smem);
+  else
+    ns_join_slabs<64>(p, m, job, smem);
 }
 
 template <int WHAT, typename O>
 __global__ __launch_bounds__(256, 2) void ns_advance_kernel(NsArgs p, int k) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int4 job = p.full[blockIdx.x];
-  const NsMat m = p.mats[job.x];
-  const int lift = ns_lift(p, job.x, k), lift_next = ns_lift(p, job.x, k + 1);
-  if (job.w == 128)
-    ns_advance<128, WHAT, O>(p, m, job.y, job.z, k, lift, lift_next, smem);
+  const NsJob job = p.full[blockIdx.x];
+  if (job.mat < 0) return;
+  const NsMat m = p.mats[job.mat];
+  const int lift = ns_lift(p, job.mat, k), lift_next = ns_lift(p, job.mat, k + 1);
+  if (job.edge == 128)
+    ns_advance<128, WHAT, O>(p, m, job, k, lift, lift_next, smem);
   else
-    ns_advance<64, WHAT, O>(p, m, job.y, job.z, k, lift, lift_next, smem);
+    ns_advance<64, WHAT, O>(p, m, job, k, lift, lift_next, smem);
 }
 
 // ---------------------------------------------------------------- host
@@ -504,14 +593,15 @@ static int ns_first(const NsArgs& a, hipStream_t st) {
 // or the parameters.
 extern "C" int dtfa_newton_schulz(const NsArgs* args, hipStream_t st) {
   const NsArgs a = *args;
-  if (a.nchunks <= 0 || a.npacks <= 0 || a.nsym <= 0 || a.nfull <= 0 || a.steps < 1) return -1;
+  if (a.nchunks <= 0 || a.npacks <= 0 || a.ngram <= 0 || a.npoly <= 0 || a.nfull <= 0 || a.steps < 1) return -1;
   if ((a.out == nullptr) == (a.w == nullptr) || (a.w != nullptr && (a.buf == nullptr || a.hyper == nullptr))) return -2;
   if (a.out == nullptr && a.dtype == IO_F16) return -3;
   int rc = a.dtype == IO_BF16 ? ns_first<bf16>(a, st) : a.dtype == IO_F16 ? ns_first<f16>(a, st)
            : a.dtype == IO_F32 ? ns_first<float>(a, st) : -3;
   for (int k = 0; k < a.steps && rc == 0; ++k) {
-    rc = ns_tiles<ns_symmetric_kernel<false>>(a.nsym, a, k, st);
-    if (rc == 0) rc = ns_tiles<ns_symmetric_kernel<true>>(a.nsym, a, k, st);
+    rc = ns_tiles<ns_symmetric_kernel<false>>(a.ngram, a, k, st);
+    if (rc == 0 && a.njoin > 0) rc = ns_tiles<ns_join_kernel>(a.njoin, a, k, st);
+    if (rc == 0) rc = ns_tiles<ns_symmetric_kernel<true>>(a.npoly, a, k, st);
     if (rc != 0) break;
     if (k + 1 < a.steps)
       rc = ns_tiles<ns_advance_kernel<NS_NEXT, float>>(a.nfull, a, k, st);

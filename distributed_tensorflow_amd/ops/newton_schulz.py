@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from typing import Dict, Optional, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -24,6 +24,9 @@ MAX_STEPS = 64
 MAX_PARTS = 1024          # partial sums of squares per matrix
 CHUNK = 8192              # elements per partial sum, at least
 
+# time of one k-step of 32 of a product tile (us, measured with the card full)
+STEP_US = {128: 0.8, 64: 0.35}
+
 # edge of the product tiles: 128 from this size of the smaller side on, 64 below
 LARGE_TILE_FROM = 512
 
@@ -33,10 +36,11 @@ _MAT = np.dtype([("at", "<i8"), ("x", "<i8"), ("a", "<i8"), ("part", "<i8"), ("r
 
 
 class NsArgs(C.Structure):
-    _fields_ = [("mats", C.c_void_p), ("chunks", C.c_void_p), ("packs", C.c_void_p), ("sym", C.c_void_p), ("full", C.c_void_p),
-                ("nchunks", C.c_int), ("npacks", C.c_int), ("nsym", C.c_int), ("nfull", C.c_int),
+    _fields_ = [("mats", C.c_void_p), ("chunks", C.c_void_p), ("packs", C.c_void_p), ("gram", C.c_void_p), ("joins", C.c_void_p),
+                ("poly", C.c_void_p), ("full", C.c_void_p), ("nchunks", C.c_int), ("npacks", C.c_int), ("ngram", C.c_int),
+                ("njoin", C.c_int), ("npoly", C.c_int), ("nfull", C.c_int),
                 ("steps", C.c_int), ("dtype", C.c_int), ("in_", C.c_void_p), ("out", C.c_void_p), ("buf", C.c_void_p),
-                ("w", C.c_void_p), ("w16", C.c_void_p), ("hyper", C.c_void_p), ("part", C.c_void_p), ("ws", C.c_void_p), ("nparts", C.c_longlong),
+                ("w", C.c_void_p), ("w16", C.c_void_p), ("hyper", C.c_void_p), ("part", C.c_void_p), ("slabs", C.c_void_p), ("ws", C.c_void_p), ("nparts", C.c_longlong),
                 ("eps", C.c_float), ("mu", C.c_float), ("wd", C.c_float), ("nesterov", C.c_int)]
 
 
@@ -47,13 +51,50 @@ def check_shape(rows: int, cols: int, what: str) -> None:
         raise ValueError("%s: %d x %d is too large (at most 2^20, the smaller side at most 2^15)" % (what, rows, cols))
 
 
-def _tiles(mat: int, rows: int, cols: int, edge: int, lower: bool = False) -> np.ndarray:
-    """{matrix, tile row, tile column, edge} of every tile, or of those on and below the diagonal."""
+def _tiles(rows: int, cols: int, lower: bool = False) -> Tuple[np.ndarray, np.ndarray]:
+    """Rows and columns of every tile of a grid, or of those on and below the diagonal, block by block of 8 x 8."""
     i, j = np.divmod(np.arange(rows * cols, dtype=np.int64), cols)
     if lower:
-        keep = j <= i
-        i, j = i[keep], j[keep]
-    return np.stack([np.full_like(i, mat), i, j, np.full_like(i, edge)], 1).astype(np.int32)
+        i, j = i[j <= i], j[j <= i]
+    order = np.lexsort((j, i, j // 8, i // 8))
+    return i[order], j[order]
+
+
+def _jobs(mat: int, i, j, edge: int, k0, k1, slab=-1) -> np.ndarray:
+    """NsJob records {matrix, tile row, tile column, edge, k0, k1, slab, -}."""
+    out = np.zeros((len(i), 8), dtype=np.int32)
+    for c, v in enumerate((mat, i, j, edge, k0, k1, slab)):
+        out[:, c] = v
+    return out
+
+
+def _cost(jobs: np.ndarray) -> np.ndarray:
+    return np.where(jobs[:, 3] == 128, STEP_US[128], STEP_US[64]) * ((jobs[:, 5] - jobs[:, 4]) // 32)
+
+
+def _over_xcds(groups: Sequence[np.ndarray]) -> np.ndarray:
+    """Workgroup n runs on XCD n % 8, each with its own L2: neighbouring tiles, which read the same rows, are dealt to the
+    XCDs in runs, longest jobs first, every run to the XCD with the least work so far; within an XCD the longest jobs
+    start first.  Shorter queues are filled up with empty jobs."""
+    total = sum(len(g) for g in groups)
+    run = max(1, min(32, total // 32))
+    runs = [g[at:at + run] for g in groups for at in range(0, len(g), run)]
+    runs.sort(key=lambda g: -float(_cost(g[:1])[0]))
+    queues: List[List[np.ndarray]] = [[] for _ in range(8)]
+    load = [0.0] * 8
+    for g in runs:
+        x = load.index(min(load))
+        queues[x].append(g)
+        load[x] += float(_cost(g).sum())
+    longest = max(sum(len(g) for g in q) for q in queues)
+    out = np.zeros((longest, 8, 8), dtype=np.int32)
+    out[:, :, 0] = -1
+    for x, q in enumerate(queues):
+        if q:
+            jobs = np.concatenate(q)
+            out[:len(jobs), x] = jobs[np.argsort(-_cost(jobs), kind="stable")]
+    out = out.reshape(-1, 8)
+    return out[:len(out) - int(np.argmax(out[::-1, 0] >= 0))]   # (no empty jobs behind the last)
 
 
 class NsPlan:
@@ -61,8 +102,8 @@ class NsPlan:
 
     def __init__(self, matrices: Sequence[Tuple[int, int, int]], device):
         mats = np.zeros(len(matrices), dtype=_MAT)
-        chunks, packs, sym, full = [], [], [], []
-        ws = part = 0
+        chunks, packs, gram, joins, poly, full = [], [], [], [], [], []
+        ws = part = slabs = 0
         for k, (at, rows, cols) in enumerate(matrices):
             check_shape(rows, cols, "orthogonalize")
             short = min(rows, cols)
@@ -78,23 +119,22 @@ class NsPlan:
             ws += 4 * rp * cp + 4 * mp * mp
             part += parts
             chunks.append(np.stack([np.full(parts, k), np.arange(parts), np.zeros(parts), np.zeros(parts)], 1).astype(np.int32))
-            packs.append(_tiles(k, rp // 64, cp // 64, 64))
-            long = max(rp, cp)
-            sym.append((-long * edge * edge, _tiles(k, mp // edge, mp // edge, edge, lower=True)))
-            full.append((-mp * edge * edge, _tiles(k, rp // edge, cp // edge, edge)))
-        # longest tiles first: the last workgroups to start are the short ones
-        sym.sort(key=lambda e: e[0])
-        full.sort(key=lambda e: e[0])
-        lists = [np.concatenate(v) for v in (chunks, packs, [t for _, t in sym], [t for _, t in full])]
+            i, j = _tiles(rp // 64, cp // 64)
+            packs.append(np.stack([np.full_like(i, k), i, j, np.zeros_like(i)], 1).astype(np.int32))
+            i, j = _tiles(mp // edge, mp // edge, lower=True)
+            gram.append(_jobs(k, i, j, edge, 0, max(rp, cp)))
+            poly.append(_jobs(k, i, j, edge, 0, mp))
+            full.append(_jobs(k, *_tiles(rp // edge, cp // edge), edge, 0, mp))
+        none = np.zeros((0, 8), dtype=np.int32)
+        lists = [np.concatenate(chunks), np.concatenate(packs), _over_xcds(gram), np.concatenate(joins + [none]),
+                 _over_xcds(poly), _over_xcds(full)]
         self.counts = [len(v) for v in lists]
-        head = mats.tobytes()
-        head += b"\0" * (-len(head) % 16)   # the lists are read 16 bytes at a time
-        blob = b"".join([head] + [v.tobytes() for v in lists])
-        host = torch.from_numpy(np.frombuffer(blob, dtype=np.uint8).copy())
-        self.table = host.to(device)
-        starts = np.cumsum([0, len(head)] + [v.nbytes for v in lists])
-        self.places = [self.table.data_ptr() + int(s) for s in starts[:5]]
-        self.ws_elems, self.parts, self.mats = ws, part, len(matrices)
+        # 32-byte aligned: the lists are read 16 and 32 bytes at a time
+        blobs = [v.tobytes() + b"\0" * (-v.nbytes % 32) for v in [mats] + lists]
+        self.table = torch.from_numpy(np.frombuffer(b"".join(blobs), dtype=np.uint8).copy()).to(device)
+        starts = np.cumsum([0] + [len(v) for v in blobs])
+        self.places = [self.table.data_ptr() + int(s) for s in starts[:7]]
+        self.ws_elems, self.parts, self.mats, self.slabs = ws, part, len(matrices), slabs
 
     def launch(self, *, inp: torch.Tensor, steps: int, out=None, buf=None, w=None, w16=None, hyper=None, mu=0.0,
                nesterov=False, wd=0.0) -> None:
@@ -102,10 +142,10 @@ class NsPlan:
         with hipk.device_of(inp):
             ws = torch.empty(self.ws_elems, dtype=torch.float16, device=dev)
             part = torch.empty(self.parts + self.mats, dtype=torch.float64, device=dev)
+            slabs = torch.empty(self.slabs * 4096, dtype=F32, device=dev) if self.slabs else None
             args = NsArgs(*self.places, *self.counts, steps, DTYPES[inp.dtype], inp.data_ptr(), hipk.ptr(out), hipk.ptr(buf),
-                          hipk.ptr(w), hipk.ptr(w16), hipk.ptr(hyper), part.data_ptr(), ws.data_ptr(),
-                          self.parts, NORM_EPS, mu, wd,
-                          1 if nesterov else 0)
+                          hipk.ptr(w), hipk.ptr(w16), hipk.ptr(hyper), part.data_ptr(), hipk.ptr(slabs), ws.data_ptr(),
+                          self.parts, NORM_EPS, mu, wd, 1 if nesterov else 0)
             hipk.check(hipk.lib().dtfa_newton_schulz(C.byref(args), hipk.stream()), "newton_schulz")
 
 

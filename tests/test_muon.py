@@ -73,10 +73,10 @@ def test_plan_covers_every_tile_once_and_stays_inside(shapes):
     table, base = plan.table.numpy(), plan.table.data_ptr()
     mats = table[:len(shapes) * ns._MAT.itemsize].view(ns._MAT)
     lists = []
-    for start, count in zip(plan.places[1:], plan.counts):
-        assert (start - base) % 16 == 0 and start - base + 16 * count <= table.size
-        lists.append(table[start - base:start - base + 16 * count].view(np.int32).reshape(-1, 4))
-    chunks, packs, sym, full = lists
+    for start, count, width in zip(plan.places[1:], plan.counts, (4, 4, 8, 8, 8, 8)):
+        assert (start - base) % 32 == 0 and start - base + 4 * width * count <= table.size
+        lists.append(table[start - base:start - base + 4 * width * count].view(np.int32).reshape(-1, width))
+    chunks, packs, gram, joins, poly, full = lists
     end = part = 0
     for k, (m, (at, r, c)) in enumerate(zip(mats, places)):
         edge = 128 if min(r, c) >= ns.LARGE_TILE_FROM else 64
@@ -91,13 +91,15 @@ def test_plan_covers_every_tile_once_and_stays_inside(shapes):
         assert sorted(map(tuple, chunks[chunks[:, 0] == k][:, 1:2])) == [(i,) for i in range(m["parts"])]
         assert {tuple(t) for t in packs[packs[:, 0] == k][:, 1:3]} == \
             {(i, j) for i in range(m["rp"] // 64) for j in range(m["cp"] // 64)}
-        n = m["mp"] // edge
-        mine = sym[sym[:, 0] == k]
-        assert (mine[:, 3] == edge).all() and len(mine) == n * (n + 1) // 2
-        assert {tuple(t) for t in mine[:, 1:3]} == {(i, j) for i in range(n) for j in range(i + 1)}
-        mine = full[full[:, 0] == k]
-        assert (mine[:, 3] == edge).all() and len(mine) == m["rp"] // edge * (m["cp"] // edge)
-        assert {tuple(t) for t in mine[:, 1:3]} == {(i, j) for i in range(m["rp"] // edge) for j in range(m["cp"] // edge)}
+        for jobs, longest, lower in ((gram, max(m["rp"], m["cp"]), True), (poly, m["mp"], True), (full, m["mp"], False)):
+            seen = np.zeros((m["mp"], m["mp"]) if lower else (m["rp"], m["cp"]), dtype=np.int64)
+            for _, ti, tj, e, k0, k1, slab, _ in jobs[jobs[:, 0] == k]:
+                assert e in (64, edge) and 0 <= k0 < k1 <= longest and k0 % 32 == k1 % 32 == 0
+                assert e * (ti + 1) <= seen.shape[0] and e * (tj + 1) <= seen.shape[1] and ti >= 0 <= tj
+                seen[e * ti:e * (ti + 1), e * tj:e * (tj + 1)] += k1 - k0
+                if lower and ti != tj:   # the mirror image
+                    seen[e * tj:e * (tj + 1), e * ti:e * (ti + 1)] += k1 - k0
+            assert (seen == longest).all()
         # the scale: a power of two, no entry of X (at most 1.21) above fp16's range
         assert math.log2(m["scale"]) == int(math.log2(m["scale"])) and 1.21 * m["scale"] < 65504
         assert m["scale"] <= math.sqrt(r * c) < 2 * m["scale"] or m["scale"] == 2 ** 15
