@@ -22,7 +22,8 @@
 // A and B are symmetric: only tiles on and below the diagonal are computed, their mirror images are copies.  All
 // matrices of an optimizer step (or of a batch) go through each stage in one launch, from work lists that name (matrix,
 // tile row, tile column), longest first.  The operands live in a workspace whose planes are padded with zeros to whole
-// tiles, so the products need no bounds checks.
+// tiles, so the products need no bounds checks; a row holds its two planes in turns of 32 values, hi then lo, so that the
+// 32 k of a step are one 128-byte line per row (apart, each plane's 64 bytes fetched a line of which half was used).
 #include "row_io.h"
 
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
@@ -36,8 +37,8 @@ typedef f16 f16x4 __attribute__((ext_vector_type(4)));
 // One matrix.  Offsets in elements of the buffer they point into.
 struct NsMat {
   long long at;    // of the matrix in the input / output / parameter buffers (rows * cols contiguous values)
-  long long x;     // four planes [rp][cp] in the workspace: X hi, X lo, next X hi, next X lo
-  long long a;     // four planes [mp][mp]: A hi, A lo, B hi, B lo
+  long long x;     // X and the next X in the workspace: two plane pairs [rp][cp]
+  long long a;     // A and B: two plane pairs [mp][mp]
   long long part;  // first of its `parts` partial sums of squares
   int rows, cols;
   int rp, cp, mp;  // padded rows, columns and min(rows, cols)
@@ -137,6 +138,29 @@ __device__ __forceinline__ void ns_split(float v, f16& hi, f16& lo) {
   lo = (f16)(v - (float)hi);
 }
 
+// A plane pair [rows][ld]: the hi value (row, col); its lo value is 32 further on.
+__device__ __forceinline__ size_t ns_at(int ld, int row, int col) {
+  return (size_t)row * 2 * ld + ((col >> 5) << 6) + (col & 31);
+}
+// eight consecutive values of a row, col a multiple of 8
+__device__ __forceinline__ void ns_get(const f16* at, float (&v)[8]) {
+  const f16x8 h = *(const f16x8*)at, l = *(const f16x8*)(at + 32);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = (float)h[j] + (float)l[j];
+}
+__device__ __forceinline__ void ns_put(f16* at, const float (&v)[8]) {
+  f16x8 h, l;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    f16 a, b;
+    ns_split(v[j], a, b);
+    h[j] = a;
+    l[j] = b;
+  }
+  *(f16x8*)at = h;
+  *(f16x8*)(at + 32) = l;
+}
+
 // X_0 times S as two fp16 planes, zeros in the padding.  A workgroup writes 64 x 64 values.
 template <typename T, bool MOMENTUM>
 __global__ __launch_bounds__(256) void ns_pack_kernel(NsArgs p) {
@@ -159,8 +183,7 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(NsArgs p) {
   const T* in = (const T*)p.in + m.at;
   const float* buf = MOMENTUM ? p.buf + m.at : nullptr;
   const float gs = MOMENTUM ? p.hyper[1] : 1.f;
-  f16* hi = p.ws + m.x;
-  f16* lo = hi + (size_t)m.rp * m.cp;
+  f16* x = p.ws + m.x;
   const int col = job.z * 64 + (threadIdx.x & 7) * 8;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -176,35 +199,26 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(NsArgs p) {
         for (int j = 0; j < 8; ++j) g[j] = ns_direction(g[j] * gs, b[j], p.mu, p.nesterov);
       }
     }
-    f16x8 vh, vl;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      f16 a, c;
-      ns_split((float)((double)g[j] * scale), a, c);
-      vh[j] = a;
-      vl[j] = c;
-    }
-    *(f16x8*)(hi + (size_t)row * m.cp + col) = vh;
-    *(f16x8*)(lo + (size_t)row * m.cp + col) = vl;
+    for (int j = 0; j < 8; ++j) g[j] = (float)((double)g[j] * scale);
+    ns_put(x + ns_at(m.cp, row, col), g);
   }
 }
 
 // ---------------------------------------------------------------- products
 #define NS_BK 32
 
-// 16-byte slot of a tile row's logical chunk: rows of 64 bytes (k contiguous) ...
-__device__ __forceinline__ int ns_swz(int row) { return (row >> 2) & 3; }
-// ... and rows of T fp16 (k is the row), as the transposing reads want it: they touch 64 bytes in each of four rows
-template <int T>
-__device__ __forceinline__ int ns_swz_tr(int row) {
-  return T == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
-}
+// Tiles in LDS.  k contiguous: T rows of 128 bytes, 16-byte chunk plane * 4 + k / 8 at slot chunk ^ ns_swz(row): 16 rows
+// reading the same chunk touch every bank once.
+__device__ __forceinline__ int ns_swz(int row) { return (row >> 1) & 7; }
+// k is the row: 32 rows of 4 T bytes, blocks of 32 columns hi and lo in turn; a transposing read touches 64 bytes in each of
+// four consecutive rows, which all start at bank 0.
+__device__ __forceinline__ int ns_swz_tr(int row) { return (row & 3) << 2; }
 
-// An operand of a product: two planes [rows][ld], element (i, k) of the operand at row i, column k (KMAJOR false) or at
-// row k, column i (KMAJOR true); `i0` is the tile's first i.
+// An operand of a product: a plane pair; element (i, k) of the operand at row i, column k, or (k-major) at row k,
+// column i; `i0` is the tile's first i.
 struct NsOperand {
-  const f16* hi;
-  const f16* lo;
+  const f16* base;
   int ld;
   int i0;
 };
@@ -214,78 +228,85 @@ struct NsOperand {
 // j = v * 32 + (e & 3) + 8 (e >> 2) + 4 (l >> 5) of row i = u * 32 + (l & 31), so four consecutive elements are four
 // consecutive columns.
 //
-// k advances by 32; each of the four waves brings one plane of the next k-tiles (P hi, P lo, Q hi, Q lo) into LDS by
+// k advances by 32; each of the four waves brings half of an operand of the next k-tiles (P, P, Q, Q) into LDS by
 // LDS-DMA, NST - 1 k-tiles ahead, with counted waits and raw barriers; the fragments of the next 16 k are read while the
 // matrix instructions of the present ones run.
 template <int T, bool PK, bool QK>
 __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& Q, int k0, int k1, char* smem,
                                            f32x16 (&acc)[T / 64][T / 64]) {
-  constexpr int PLANE = T * NS_BK * 2;        // bytes
-  constexpr int STAGE = 4 * PLANE;
+  constexpr int OPER = T * NS_BK * 4;         // bytes of an operand's k-tile, both planes
+  constexpr int STAGE = 2 * OPER;
   constexpr int NST = T == 128 ? 2 : 4;
-  constexpr int LPS = PLANE / 1024;           // LDS-DMA instructions per wave and k-tile
+  constexpr int LPS = OPER / 2048;            // LDS-DMA instructions per wave and k-tile
   constexpr int MT = T / 64;
   const int lane = threadIdx.x & 63;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wid >> 1, wc = wid & 1;
 
-  // staging: this wave's plane
+  // staging: this wave's half of an operand
   const bool kmajor = wid < 2 ? PK : QK;
-  const f16* plane = wid == 0 ? P.hi : wid == 1 ? P.lo : wid == 2 ? Q.hi : Q.lo;
+  const f16* base = wid < 2 ? P.base : Q.base;
   const int ld = wid < 2 ? P.ld : Q.ld, i0 = wid < 2 ? P.i0 : Q.i0;
-  const f16* src;
-  size_t inst, step;  // elements between the rows of two instructions, between two k-tiles
+  const f16* src[2];  // of the even and of the odd instructions
+  size_t pair, step;  // elements between the rows of two instructions, between two k-tiles
   if (kmajor) {
-    constexpr int RPI = 1024 / (T * 2);       // k rows per instruction
-    const int r = lane / (64 / RPI), slot = lane % (64 / RPI);
-    src = plane + (size_t)(k0 + r) * ld + i0 + ((slot ^ ns_swz_tr<T>(r)) << 3);
-    // (an instruction covers 4 or 8 rows and the swizzle has period 4: the slot is the same for all of them)
-    inst = (size_t)RPI * ld;
-    step = (size_t)NS_BK * ld;
-  } else {
-    const int r = lane >> 2, slot = lane & 3; // 16 rows per instruction, the swizzle has period 16
-    src = plane + (size_t)(i0 + r) * ld + k0 + ((slot ^ ns_swz(r)) << 3);
-    inst = (size_t)16 * ld;
-    step = NS_BK;
-  }
-  auto stage = [&](int buf) {
-    char* dst = smem + buf * STAGE + wid * PLANE;
+    constexpr int RPI = 256 / T;              // k rows per instruction: 2 or 4; this wave brings 16
 #pragma unroll
-    for (int i = 0; i < LPS; ++i) glds16_untracked(src + i * inst, dst + i * 1024);
-    src += step;
+    for (int o = 0; o < 2; ++o) {
+      const int r = (wid & 1) * 16 + o * RPI + lane / (64 / RPI), slot = lane % (64 / RPI);
+      src[o] = base + (size_t)(k0 + r) * 2 * ld + 2 * i0 + ((slot ^ ns_swz_tr(r)) << 3);
+    }
+    pair = (size_t)4 * RPI * ld;
+    step = (size_t)NS_BK * 2 * ld;
+  } else {
+#pragma unroll
+    for (int o = 0; o < 2; ++o) {             // 8 rows per instruction
+      const int r = (wid & 1) * (T / 2) + o * 8 + (lane >> 3), slot = lane & 7;
+      src[o] = base + (size_t)(i0 + r) * 2 * ld + 2 * k0 + ((slot ^ ns_swz(r)) << 3);
+    }
+    pair = (size_t)32 * ld;
+    step = 2 * NS_BK;
+  }
+  // (the swizzles repeat every 16 rows, or 4: every second instruction finds the same slots)
+  auto stage = [&](int buf) {
+    char* dst = smem + buf * STAGE + wid * (OPER / 2);
+#pragma unroll
+    for (int i = 0; i < LPS; ++i) glds16_untracked(src[i & 1] + (i >> 1) * pair, dst + i * 1024);
+    src[0] += step;
+    src[1] += step;
   };
 
   // fragments
   const int tr_q = (lane & 15) >> 2;
   const int tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
   const int tr_k = 8 * (lane >> 5) + tr_q;
-  auto frag = [&](const char* plane_lds, bool km, int row0, int ks) -> f16x8 {
+  auto frag = [&](const char* oper, bool km, int row0, int ks, int lo) -> f16x8 {
     if (km) {
-      const int col = row0 + tr_col;
       union { s16x4 h[2]; f16x8 v; } r;
+      const int chunk = (row0 >> 5) * 8 + lo * 4 + (tr_col >> 3);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         const int krow = ks * 16 + tr_k + 4 * q;
-        const char* at = plane_lds + krow * (T * 2) + (((col >> 3) ^ ns_swz_tr<T>(krow)) << 4) + (col & 7) * 2;
+        const char* at = oper + krow * (T * 4) + ((chunk ^ ns_swz_tr(krow)) << 4) + (tr_col & 7) * 2;
         r.h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)at);
       }
       return r.v;
     }
     const int row = row0 + (lane & 31);
-    return *(const f16x8*)(plane_lds + row * 64 + (((ks * 2 + (lane >> 5)) ^ ns_swz(row)) << 4));
+    return *(const f16x8*)(oper + row * 128 + (((lo * 4 + ks * 2 + (lane >> 5)) ^ ns_swz(row)) << 4));
   };
   f16x8 ph[2][MT], pl[2][MT], qh[2][MT], ql[2][MT];
   auto load_frags = [&](int buf, int ks, int to) {
-    const char* base = smem + buf * STAGE;
+    const char* at = smem + buf * STAGE;
 #pragma unroll
     for (int u = 0; u < MT; ++u) {
-      ph[to][u] = frag(base, PK, wr * (T / 2) + u * 32, ks);
-      qh[to][u] = frag(base + 2 * PLANE, QK, wc * (T / 2) + u * 32, ks);
+      ph[to][u] = frag(at, PK, wr * (T / 2) + u * 32, ks, 0);
+      qh[to][u] = frag(at + OPER, QK, wc * (T / 2) + u * 32, ks, 0);
     }
 #pragma unroll
     for (int u = 0; u < MT; ++u) {
-      ql[to][u] = frag(base + 3 * PLANE, QK, wc * (T / 2) + u * 32, ks);
-      pl[to][u] = frag(base + PLANE, PK, wr * (T / 2) + u * 32, ks);
+      ql[to][u] = frag(at + OPER, QK, wc * (T / 2) + u * 32, ks, 1);
+      pl[to][u] = frag(at, PK, wr * (T / 2) + u * 32, ks, 1);
     }
   };
   auto multiply = [&](int from) {
@@ -369,24 +390,6 @@ __device__ __forceinline__ void ns_to_lds(const f32x16 (&acc)[T / 64][T / 64], f
   __syncthreads();
 }
 
-__device__ __forceinline__ void ns_join(const f16* hi, const f16* lo, float (&v)[8]) {
-  const f16x8 h = *(const f16x8*)hi, l = *(const f16x8*)lo;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = (float)h[j] + (float)l[j];
-}
-__device__ __forceinline__ void ns_put(f16* hi, f16* lo, const float (&v)[8]) {
-  f16x8 h, l;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    f16 a, b;
-    ns_split(v[j], a, b);
-    h[j] = a;
-    l[j] = b;
-  }
-  *(f16x8*)hi = h;
-  *(f16x8*)lo = l;
-}
-
 // e_k of a matrix
 __device__ __forceinline__ int ns_lift(const NsArgs& p, int mat, int k) {
   const int e = (int)p.part[p.nparts + mat] - 2 * k;
@@ -396,21 +399,20 @@ __device__ __forceinline__ int ns_lift(const NsArgs& p, int mat, int k) {
 // The fp32 tile in LDS, sums over all k, becomes the tile of A, or with POLY of B = b A + c A A, and its mirror image.
 template <int T, bool POLY>
 __device__ __forceinline__ void ns_symmetric_out(const NsArgs& p, const NsMat& m, int ti, int tj, int lift, float* tile) {
-  const size_t as = (size_t)m.mp * m.mp;
   f16* a = p.ws + m.a;
-  f16* out = POLY ? a + 2 * as : a;
+  f16* out = POLY ? a + (size_t)2 * m.mp * m.mp : a;
   const int i0 = ti * T, j0 = tj * T;
   const float f = POLY ? ldexpf(NS_C / NS_GRAM_SCALE, -2 * lift) : NS_GRAM_SCALE / (m.scale * m.scale);
   // rows of the tile: eight consecutive columns a thread
   for (int e = threadIdx.x; e < T * T / 8; e += 256) {
     const int r = e / (T / 8), c = e % (T / 8) * 8;
-    const size_t at = (size_t)(i0 + r) * m.mp + j0 + c;
+    const size_t at = ns_at(m.mp, i0 + r, j0 + c);
     float* t = tile + r * NS_PITCH(T) + c;
     float v[8];
-    if (POLY) ns_join(a + at, a + as + at, v);
+    if (POLY) ns_get(a + at, v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = POLY ? NS_B * v[j] + f * t[j] : f * t[j];
-    ns_put(out + at, out + as + at, v);
+    ns_put(out + at, v);
     if (ti != tj)
 #pragma unroll
       for (int j = 0; j < 8; ++j) t[j] = v[j];
@@ -423,8 +425,7 @@ __device__ __forceinline__ void ns_symmetric_out(const NsArgs& p, const NsMat& m
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = tile[(r + j) * NS_PITCH(T) + c];
-    const size_t at = (size_t)(j0 + c) * m.mp + i0 + r;
-    ns_put(out + at, out + as + at, v);
+    ns_put(out + ns_at(m.mp, j0 + c, i0 + r), v);
   }
 }
 
@@ -432,16 +433,15 @@ __device__ __forceinline__ void ns_symmetric_out(const NsArgs& p, const NsMat& m
 template <int T, bool POLY>
 __device__ __forceinline__ void ns_symmetric(const NsArgs& p, const NsMat& m, const NsJob& job, int k, int lift, char* smem) {
   f32x16 acc[T / 64][T / 64];
-  const size_t xs = (size_t)m.rp * m.cp, as = (size_t)m.mp * m.mp;
-  const f16* x = p.ws + m.x + (k & 1 ? 2 * xs : 0);
+  const f16* x = p.ws + m.x + (k & 1 ? (size_t)2 * m.rp * m.cp : 0);
   const f16* a = p.ws + m.a;
   const int i0 = job.ti * T, j0 = job.tj * T;
   if (POLY)
-    ns_product<T, false, false>({a, a + as, m.mp, i0}, {a, a + as, m.mp, j0}, job.k0, job.k1, smem, acc);
+    ns_product<T, false, false>({a, m.mp, i0}, {a, m.mp, j0}, job.k0, job.k1, smem, acc);
   else if (m.tall)
-    ns_product<T, true, true>({x, x + xs, m.cp, i0}, {x, x + xs, m.cp, j0}, job.k0, job.k1, smem, acc);
+    ns_product<T, true, true>({x, m.cp, i0}, {x, m.cp, j0}, job.k0, job.k1, smem, acc);
   else
-    ns_product<T, false, false>({x, x + xs, m.cp, i0}, {x, x + xs, m.cp, j0}, job.k0, job.k1, smem, acc);
+    ns_product<T, false, false>({x, m.cp, i0}, {x, m.cp, j0}, job.k0, job.k1, smem, acc);
   float* tile = (float*)smem;
   ns_to_lds<T>(acc, tile);
   if (!POLY && job.slab >= 0) {
@@ -478,15 +478,15 @@ template <int T, int WHAT, typename O>
 __device__ __forceinline__ void ns_advance(const NsArgs& p, const NsMat& m, const NsJob& job, int k, int lift, int lift_next,
                                            char* smem) {
   f32x16 acc[T / 64][T / 64];
-  const size_t xs = (size_t)m.rp * m.cp, as = (size_t)m.mp * m.mp;
-  const f16* x = p.ws + m.x + (k & 1 ? 2 * xs : 0);
-  f16* next = p.ws + m.x + (k & 1 ? 0 : 2 * xs);
-  const f16* b = p.ws + m.a + 2 * as;
+  const size_t xs = (size_t)2 * m.rp * m.cp;
+  const f16* x = p.ws + m.x + (k & 1 ? xs : 0);
+  f16* next = p.ws + m.x + (k & 1 ? 0 : xs);
+  const f16* b = p.ws + m.a + (size_t)2 * m.mp * m.mp;
   const int i0 = job.ti * T, j0 = job.tj * T;
   if (m.tall)
-    ns_product<T, false, false>({x, x + xs, m.cp, i0}, {b, b + as, m.mp, j0}, job.k0, job.k1, smem, acc);
+    ns_product<T, false, false>({x, m.cp, i0}, {b, m.mp, j0}, job.k0, job.k1, smem, acc);
   else
-    ns_product<T, false, true>({b, b + as, m.mp, i0}, {x, x + xs, m.cp, j0}, job.k0, job.k1, smem, acc);
+    ns_product<T, false, true>({b, m.mp, i0}, {x, m.cp, j0}, job.k0, job.k1, smem, acc);
   float* tile = (float*)smem;
   ns_to_lds<T>(acc, tile);
   const float lr = WHAT == NS_APPLY ? p.hyper[0] : 0.f;
@@ -498,14 +498,14 @@ __device__ __forceinline__ void ns_advance(const NsArgs& p, const NsMat& m, cons
     const int r = e / (T / 8), c = e % (T / 8) * 8;
     const int row = i0 + r, col = j0 + c;
     if (WHAT != NS_NEXT && (row >= m.rows || col >= m.cols)) continue;
-    const size_t at = (size_t)row * m.cp + col;
+    const size_t at = ns_at(m.cp, row, col);
     const float* t = tile + r * NS_PITCH(T) + c;
     float v[8];
-    ns_join(x + at, x + xs + at, v);
+    ns_get(x + at, v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = fx * v[j] + ft * t[j];
     if (WHAT == NS_NEXT) {
-      ns_put(next + at, next + xs + at, v);
+      ns_put(next + at, v);
       continue;
     }
 #pragma unroll
