@@ -51,7 +51,7 @@ struct NsMat {
 
 // One workgroup of a product stage: the tile (ti, tj) of `edge` x `edge` values, summed over k0 <= k < k1.  Where the
 // reduction is cut in several jobs, each leaves its fp32 sums in slab `slab` (in units of 64 x 64 values), else -1; the
-// job that joins them (NsArgs::gram_joins) has the first one's number and k0 = how many there are.
+// job that joins them (NsArgs::gram_joins, poly_joins) has the first one's number and k0 = how many there are.
 struct NsJob {
   int mat;  // -1: nothing (the lists are interleaved from eight queues of equal length)
   int ti, tj, edge;
@@ -66,10 +66,11 @@ struct NsArgs {
   const NsJob* gram;        // tiles of A, tj <= ti
   const NsJob* gram_joins;
   const NsJob* poly;        // tiles of B, tj <= ti
+  const NsJob* poly_joins;
   const NsJob* full;        // tiles of X
-  int nchunks, npacks, ngram, njoin, npoly, nfull;
+  int nchunks, npacks, ngram, ngram_joins, npoly, npoly_joins, nfull;
   int steps;
-  int dtype;           // of `in` (and `out`): IO_*
+  int dtype, pad;      // of `in` (and `out`): IO_*
   const void* in;      // the matrices, or their gradients
   void* out;           // orthogonalised matrices (null: parameter update)
   float* buf;          // momentum (null: none)
@@ -444,7 +445,7 @@ __device__ __forceinline__ void ns_symmetric(const NsArgs& p, const NsMat& m, co
     ns_product<T, false, false>({x, m.cp, i0}, {x, m.cp, j0}, job.k0, job.k1, smem, acc);
   float* tile = (float*)smem;
   ns_to_lds<T>(acc, tile);
-  if (!POLY && job.slab >= 0) {
+  if (job.slab >= 0) {
     float* slab = p.slabs + (size_t)job.slab * 4096;
     for (int e = threadIdx.x; e < T * T / 4; e += 256)
       *(f32x4*)(slab + e * 4) = *(const f32x4*)(tile + e / (T / 4) * NS_PITCH(T) + e % (T / 4) * 4);
@@ -454,8 +455,8 @@ __device__ __forceinline__ void ns_symmetric(const NsArgs& p, const NsMat& m, co
 }
 
 // Sums of the slabs of a tile, in order.
-template <int T>
-__device__ __forceinline__ void ns_join_slabs(const NsArgs& p, const NsMat& m, const NsJob& job, char* smem) {
+template <int T, bool POLY>
+__device__ __forceinline__ void ns_join_slabs(const NsArgs& p, const NsMat& m, const NsJob& job, int lift, char* smem) {
   float* tile = (float*)smem;
   const float* slab = p.slabs + (size_t)job.slab * 4096;
   for (int e = threadIdx.x; e < T * T / 4; e += 256) {
@@ -468,7 +469,7 @@ __device__ __forceinline__ void ns_join_slabs(const NsArgs& p, const NsMat& m, c
     *(f32x4*)(tile + e / (T / 4) * NS_PITCH(T) + e % (T / 4) * 4) = v;
   }
   __syncthreads();
-  ns_symmetric_out<T, false>(p, m, job.ti, job.tj, 0, tile);
+  ns_symmetric_out<T, POLY>(p, m, job.ti, job.tj, lift, tile);
 }
 
 enum { NS_NEXT = 0, NS_OUT = 1, NS_APPLY = 2 };
@@ -537,14 +538,16 @@ __global__ __launch_bounds__(256, 2) void ns_symmetric_kernel(NsArgs p, int k) {
     ns_symmetric<64, POLY>(p, m, job, k, lift, smem);
 }
 
-__global__ __launch_bounds__(256, 2) void ns_join_kernel(NsArgs p, int) {
+template <bool POLY>
+__global__ __launch_bounds__(256, 2) void ns_join_kernel(NsArgs p, int k) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const NsJob job = p.gram_joins[blockIdx.x];
+  const NsJob job = (POLY ? p.poly_joins : p.gram_joins)[blockIdx.x];
   const NsMat m = p.mats[job.mat];
+  const int lift = POLY ? ns_lift(p, job.mat, k) : 0;
   if (job.edge == 128)
-    ns_join_slabs<128>(p, m, job, smem);
+    ns_join_slabs<128, POLY>(p, m, job, lift, smem);
   else
-    ns_join_slabs<64>(p, m, job, smem);
+    ns_join_slabs<64, POLY>(p, m, job, lift, smem);
 }
 
 template <int WHAT, typename O>
@@ -600,8 +603,9 @@ extern "C" int dtfa_newton_schulz(const NsArgs* args, hipStream_t st) {
            : a.dtype == IO_F32 ? ns_first<float>(a, st) : -3;
   for (int k = 0; k < a.steps && rc == 0; ++k) {
     rc = ns_tiles<ns_symmetric_kernel<false>>(a.ngram, a, k, st);
-    if (rc == 0 && a.njoin > 0) rc = ns_tiles<ns_join_kernel>(a.njoin, a, k, st);
+    if (rc == 0 && a.ngram_joins > 0) rc = ns_tiles<ns_join_kernel<false>>(a.ngram_joins, a, k, st);
     if (rc == 0) rc = ns_tiles<ns_symmetric_kernel<true>>(a.npoly, a, k, st);
+    if (rc == 0 && a.npoly_joins > 0) rc = ns_tiles<ns_join_kernel<true>>(a.npoly_joins, a, k, st);
     if (rc != 0) break;
     if (k + 1 < a.steps)
       rc = ns_tiles<ns_advance_kernel<NS_NEXT, float>>(a.nfull, a, k, st);

@@ -24,11 +24,14 @@ MAX_STEPS = 64
 MAX_PARTS = 1024          # partial sums of squares per matrix
 CHUNK = 8192              # elements per partial sum, at least
 
-# time of one k-step of 32 of a product tile (us, measured with the card full)
-STEP_US = {128: 0.8, 64: 0.35}
-
-# edge of the product tiles: 128 from this size of the smaller side on, 64 below
-LARGE_TILE_FROM = 512
+# Measured on one MI355X, a CU's time in us: a tile job's fixed part (its first loads, the epilogue) and a k-step of 32.
+# A 128 x 128 tile does four times the work of a 64 x 64 tile in twice the time, so large tiles win once there are enough
+# of them for 256 CUs.
+JOB_US = {128: 4.0, 64: 2.0}
+STEP_US = {128: 0.72, 64: 0.36}
+CUS = 256
+SLOTS = 2 * CUS           # workgroups at a time
+MIN_STEPS = 8             # shortest piece of a cut reduction
 
 _MAT = np.dtype([("at", "<i8"), ("x", "<i8"), ("a", "<i8"), ("part", "<i8"), ("rows", "<i4"), ("cols", "<i4"),
                  ("rp", "<i4"), ("cp", "<i4"), ("mp", "<i4"), ("parts", "<i4"), ("chunk", "<i4"), ("tall", "<i4"),
@@ -37,9 +40,9 @@ _MAT = np.dtype([("at", "<i8"), ("x", "<i8"), ("a", "<i8"), ("part", "<i8"), ("r
 
 class NsArgs(C.Structure):
     _fields_ = [("mats", C.c_void_p), ("chunks", C.c_void_p), ("packs", C.c_void_p), ("gram", C.c_void_p), ("joins", C.c_void_p),
-                ("poly", C.c_void_p), ("full", C.c_void_p), ("nchunks", C.c_int), ("npacks", C.c_int), ("ngram", C.c_int),
-                ("njoin", C.c_int), ("npoly", C.c_int), ("nfull", C.c_int),
-                ("steps", C.c_int), ("dtype", C.c_int), ("in_", C.c_void_p), ("out", C.c_void_p), ("buf", C.c_void_p),
+                ("poly", C.c_void_p), ("poly_joins", C.c_void_p), ("full", C.c_void_p), ("nchunks", C.c_int),
+                ("npacks", C.c_int), ("ngram", C.c_int), ("ngram_joins", C.c_int), ("npoly", C.c_int),
+                ("npoly_joins", C.c_int), ("nfull", C.c_int), ("steps", C.c_int), ("dtype", C.c_int), ("pad", C.c_int), ("in_", C.c_void_p), ("out", C.c_void_p), ("buf", C.c_void_p),
                 ("w", C.c_void_p), ("w16", C.c_void_p), ("hyper", C.c_void_p), ("part", C.c_void_p), ("slabs", C.c_void_p), ("ws", C.c_void_p), ("nparts", C.c_longlong),
                 ("eps", C.c_float), ("mu", C.c_float), ("wd", C.c_float), ("nesterov", C.c_int)]
 
@@ -68,8 +71,63 @@ def _jobs(mat: int, i, j, edge: int, k0, k1, slab=-1) -> np.ndarray:
     return out
 
 
+def _job_us(edge: int, steps: float) -> float:
+    return JOB_US[edge] + STEP_US[edge] * steps
+
+
 def _cost(jobs: np.ndarray) -> np.ndarray:
-    return np.where(jobs[:, 3] == 128, STEP_US[128], STEP_US[64]) * ((jobs[:, 5] - jobs[:, 4]) // 32)
+    large = jobs[:, 3] == 128
+    return (np.where(large, JOB_US[128], JOB_US[64])
+            + np.where(large, STEP_US[128], STEP_US[64]) * ((jobs[:, 5] - jobs[:, 4]) // 32))
+
+
+def _up(v: int, edge: int) -> int:
+    return -(-v // edge) * edge
+
+
+def _span(counts_costs) -> float:
+    """Time of a launch of (count, cost) jobs: an even share per CU plus what the last jobs, which are the short ones,
+    leave idle; never less than the longest job."""
+    total = sum(n * c for n, c in counts_costs)
+    longest = max(c for _, c in counts_costs)
+    return max(longest, total / CUS + 0.4 * longest)
+
+
+def _choose(dims: Sequence[Tuple[int, int, int]], symmetric: bool) -> Tuple[int, int]:
+    """(size of the shorter of tile rows / columns from which tiles are 128, longest piece of a reduction in k-steps) of a
+    stage whose outputs are ``rows x cols`` sums over ``K`` for (rows, cols, K) in ``dims``."""
+    best = (math.inf, 0, 0)
+    for large_from in (128, 256, 512, 1024, 1 << 30):
+        for piece in (1 << 30, 64, 32, 16, MIN_STEPS) if symmetric else (1 << 30,):
+            jobs, slabs = [], 0
+            for rows, cols, K in dims:
+                edge = 128 if min(rows, cols) >= large_from else 64
+                tr, tc, steps = -(-rows // edge), -(-cols // edge), _up(K, edge) // 32
+                n = tr * (tr + 1) // 2 if symmetric else tr * tc
+                cut = -(-steps // piece)
+                jobs.append((n * cut, _job_us(edge, -(-steps // cut))))
+                slabs += n * cut * edge * edge * 4 if cut > 1 else 0
+            us = _span(jobs) + (5.0 + slabs * 2 / 3e6 if slabs else 0.0)
+            if us < best[0]:
+                best = (us, large_from, piece)
+    return best[1], best[2]
+
+
+def _cut(jobs: np.ndarray, piece: int, slabs: int) -> Tuple[np.ndarray, np.ndarray, int]:
+    """Jobs with their reductions cut into pieces of at most ``piece`` k-steps, the jobs that join the slabs of those that
+    were, and the next free slab."""
+    steps = int(jobs[0, 5] - jobs[0, 4]) // 32
+    cut = -(-steps // piece)
+    if cut == 1:
+        return jobs, jobs[:0], slabs
+    unit = (int(jobs[0, 3]) // 64) ** 2
+    out = np.repeat(jobs, cut, axis=0)
+    at = np.tile(np.arange(cut), len(jobs))
+    out[:, 4], out[:, 5] = at * steps // cut * 32, (at + 1) * steps // cut * 32
+    out[:, 6] = slabs + np.arange(len(out)) * unit
+    joins = jobs.copy()
+    joins[:, 4], joins[:, 6] = cut, slabs + np.arange(len(jobs)) * cut * unit
+    return out, joins, slabs + len(out) * unit
 
 
 def _over_xcds(groups: Sequence[np.ndarray]) -> np.ndarray:
@@ -102,16 +160,20 @@ class NsPlan:
 
     def __init__(self, matrices: Sequence[Tuple[int, int, int]], device):
         mats = np.zeros(len(matrices), dtype=_MAT)
-        chunks, packs, gram, joins, poly, full = [], [], [], [], [], []
-        ws = part = slabs = 0
-        for k, (at, rows, cols) in enumerate(matrices):
+        for _, rows, cols in matrices:
             check_shape(rows, cols, "orthogonalize")
+        sides = [(min(rows, cols), max(rows, cols)) for _, rows, cols in matrices]
+        gram_large, gram_piece = _choose([(short, short, long) for short, long in sides], True)
+        poly_large, poly_piece = _choose([(short, short, short) for short, _ in sides], True)
+        full_large, _ = _choose([(short, long, short) for short, long in sides], False)
+        chunks, packs, gram, gram_joins, poly, poly_joins, full = [], [], [], [], [], [], []
+        ws = part = gram_slabs = poly_slabs = 0
+        for k, (at, rows, cols) in enumerate(matrices):
             short = min(rows, cols)
-            edge = 128 if short >= LARGE_TILE_FROM else 64
-            up = lambda v: -(-v // edge) * edge  # noqa: E731
-            rp, cp, mp = up(rows), up(cols), up(short)
+            edge = 128 if short >= min(gram_large, poly_large, full_large) else 64
+            rp, cp, mp = _up(rows, edge), _up(cols, edge), _up(short, edge)
             n = rows * cols
-            chunk = max(CHUNK, -(-n // (MAX_PARTS * CHUNK)) * CHUNK)
+            chunk = max(CHUNK, _up(-(-n // MAX_PARTS), CHUNK))
             parts = -(-n // chunk)
             scale = 2.0 ** math.floor(math.log2(min(math.sqrt(n), 2.0 ** 15)))
             mats[k] = (at, ws, ws + 4 * rp * cp, part, rows, cols, rp, cp, mp, parts, chunk, rows > cols, scale,
@@ -121,19 +183,26 @@ class NsPlan:
             chunks.append(np.stack([np.full(parts, k), np.arange(parts), np.zeros(parts), np.zeros(parts)], 1).astype(np.int32))
             i, j = _tiles(rp // 64, cp // 64)
             packs.append(np.stack([np.full_like(i, k), i, j, np.zeros_like(i)], 1).astype(np.int32))
-            i, j = _tiles(mp // edge, mp // edge, lower=True)
-            gram.append(_jobs(k, i, j, edge, 0, max(rp, cp)))
-            poly.append(_jobs(k, i, j, edge, 0, mp))
-            full.append(_jobs(k, *_tiles(rp // edge, cp // edge), edge, 0, mp))
-        none = np.zeros((0, 8), dtype=np.int32)
-        lists = [np.concatenate(chunks), np.concatenate(packs), _over_xcds(gram), np.concatenate(joins + [none]),
-                 _over_xcds(poly), _over_xcds(full)]
+            e = 128 if short >= gram_large else 64
+            tiles = _jobs(k, *_tiles(mp // e, mp // e, lower=True), e, 0, max(rp, cp))
+            jobs, joins, gram_slabs = _cut(tiles, gram_piece, gram_slabs)
+            gram.append(jobs)
+            gram_joins.append(joins)
+            e = 128 if short >= poly_large else 64
+            jobs, joins, poly_slabs = _cut(_jobs(k, *_tiles(mp // e, mp // e, lower=True), e, 0, mp), poly_piece, poly_slabs)
+            poly.append(jobs)
+            poly_joins.append(joins)
+            e = 128 if short >= full_large else 64
+            full.append(_jobs(k, *_tiles(rp // e, cp // e), e, 0, mp))
+        slabs = max(gram_slabs, poly_slabs)   # (a stage's slabs are joined before the next stage writes its own)
+        lists = [np.concatenate(chunks), np.concatenate(packs), _over_xcds(gram), np.concatenate(gram_joins),
+                 _over_xcds(poly), np.concatenate(poly_joins), _over_xcds(full)]
         self.counts = [len(v) for v in lists]
         # 32-byte aligned: the lists are read 16 and 32 bytes at a time
         blobs = [v.tobytes() + b"\0" * (-v.nbytes % 32) for v in [mats] + lists]
         self.table = torch.from_numpy(np.frombuffer(b"".join(blobs), dtype=np.uint8).copy()).to(device)
         starts = np.cumsum([0] + [len(v) for v in blobs])
-        self.places = [self.table.data_ptr() + int(s) for s in starts[:7]]
+        self.places = [self.table.data_ptr() + int(s) for s in starts[:8]]
         self.ws_elems, self.parts, self.mats, self.slabs = ws, part, len(matrices), slabs
 
     def launch(self, *, inp: torch.Tensor, steps: int, out=None, buf=None, w=None, w16=None, hyper=None, mu=0.0,
@@ -143,7 +212,7 @@ class NsPlan:
             ws = torch.empty(self.ws_elems, dtype=torch.float16, device=dev)
             part = torch.empty(self.parts + self.mats, dtype=torch.float64, device=dev)
             slabs = torch.empty(self.slabs * 4096, dtype=F32, device=dev) if self.slabs else None
-            args = NsArgs(*self.places, *self.counts, steps, DTYPES[inp.dtype], inp.data_ptr(), hipk.ptr(out), hipk.ptr(buf),
+            args = NsArgs(*self.places, *self.counts, steps, DTYPES[inp.dtype], 0, inp.data_ptr(), hipk.ptr(out), hipk.ptr(buf),
                           hipk.ptr(w), hipk.ptr(w16), hipk.ptr(hyper), part.data_ptr(), hipk.ptr(slabs), ws.data_ptr(),
                           self.parts, NORM_EPS, mu, wd, 1 if nesterov else 0)
             hipk.check(hipk.lib().dtfa_newton_schulz(C.byref(args), hipk.stream()), "newton_schulz")

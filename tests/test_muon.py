@@ -73,13 +73,14 @@ def test_plan_covers_every_tile_once_and_stays_inside(shapes):
     table, base = plan.table.numpy(), plan.table.data_ptr()
     mats = table[:len(shapes) * ns._MAT.itemsize].view(ns._MAT)
     lists = []
-    for start, count, width in zip(plan.places[1:], plan.counts, (4, 4, 8, 8, 8, 8)):
+    for start, count, width in zip(plan.places[1:], plan.counts, (4, 4, 8, 8, 8, 8, 8)):
         assert (start - base) % 32 == 0 and start - base + 4 * width * count <= table.size
         lists.append(table[start - base:start - base + 4 * width * count].view(np.int32).reshape(-1, width))
-    chunks, packs, gram, joins, poly, full = lists
+    chunks, packs, gram, gram_joins, poly, poly_joins, full = lists
     end = part = 0
+    slabs = {id(gram): [], id(poly): [], id(full): []}   # (first, length) of every tile's slabs
     for k, (m, (at, r, c)) in enumerate(zip(mats, places)):
-        edge = 128 if min(r, c) >= ns.LARGE_TILE_FROM else 64
+        edge = 128 if any((t[t[:, 0] == k][:, 3] == 128).any() for t in (gram, poly, full)) else 64
         assert (m["at"], m["rows"], m["cols"], m["tall"]) == (at, r, c, r > c)
         for padded, size in ((m["rp"], r), (m["cp"], c), (m["mp"], min(r, c))):
             assert size <= padded < size + edge and padded % edge == 0
@@ -93,17 +94,35 @@ def test_plan_covers_every_tile_once_and_stays_inside(shapes):
             {(i, j) for i in range(m["rp"] // 64) for j in range(m["cp"] // 64)}
         for jobs, longest, lower in ((gram, max(m["rp"], m["cp"]), True), (poly, m["mp"], True), (full, m["mp"], False)):
             seen = np.zeros((m["mp"], m["mp"]) if lower else (m["rp"], m["cp"]), dtype=np.int64)
+            pieces = {}
             for _, ti, tj, e, k0, k1, slab, _ in jobs[jobs[:, 0] == k]:
                 assert e in (64, edge) and 0 <= k0 < k1 <= longest and k0 % 32 == k1 % 32 == 0
                 assert e * (ti + 1) <= seen.shape[0] and e * (tj + 1) <= seen.shape[1] and ti >= 0 <= tj
                 seen[e * ti:e * (ti + 1), e * tj:e * (tj + 1)] += k1 - k0
                 if lower and ti != tj:   # the mirror image
                     seen[e * tj:e * (tj + 1), e * ti:e * (ti + 1)] += k1 - k0
+                assert (slab >= 0) == (k1 - k0 < longest)
+                pieces.setdefault((ti, tj, e), []).append((k0, k1, slab))
+            joins = {tuple(t[1:4]): (t[4], t[6]) for t in (gram_joins if jobs is gram else poly_joins) if t[0] == k} \
+                if lower else {}
+            assert set(joins) == {t for t, v in pieces.items() if len(v) > 1}
+            for tile, v in pieces.items():   # the pieces follow one another, and so do their slabs
+                v.sort()
+                assert v[0][0] == 0 and v[-1][1] == longest and all(a[1] == b[0] for a, b in zip(v, v[1:]))
+                if len(v) > 1:
+                    unit = (tile[2] // 64) ** 2
+                    assert joins[tile] == (len(v), v[0][2])
+                    assert [s for _, _, s in v] == [v[0][2] + i * unit for i in range(len(v))]
+                    slabs[id(jobs)] += [v[0][2], len(v) * unit]
             assert (seen == longest).all()
         # the scale: a power of two, no entry of X (at most 1.21) above fp16's range
         assert math.log2(m["scale"]) == int(math.log2(m["scale"])) and 1.21 * m["scale"] < 65504
         assert m["scale"] <= math.sqrt(r * c) < 2 * m["scale"] or m["scale"] == 2 ** 15
     assert plan.ws_elems == end and plan.parts == part
+    for v in slabs.values():
+        places = sorted(zip(v[::2], v[1::2]))
+        assert all(a + n == b for (a, n), (b, _) in zip(places, places[1:])) and (not places or places[0][0] == 0)
+        assert not places or sum(places[-1]) <= plan.slabs
 
 
 def _model():
