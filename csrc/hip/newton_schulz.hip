@@ -162,12 +162,29 @@ __device__ __forceinline__ void ns_put(f16* at, const float (&v)[8]) {
   *(f16x8*)(at + 32) = l;
 }
 
-// X_0 times S as two fp16 planes, zeros in the padding.  A workgroup writes 64 x 64 values.
+// X_0 times S as two fp16 planes, zeros in the padding.  A workgroup writes 64 x 64 values; its reads are on their way
+// while the norm is put together.
 template <typename T, bool MOMENTUM>
 __global__ __launch_bounds__(256) void ns_pack_kernel(NsArgs p) {
   __shared__ double red[4];
   const int4 job = p.packs[blockIdx.x];
   const NsMat m = p.mats[job.x];
+  const T* in = (const T*)p.in + m.at;
+  const float* buf = MOMENTUM ? p.buf + m.at : nullptr;
+  const float gs = MOMENTUM ? p.hyper[1] : 1.f;
+  f16* x = p.ws + m.x;
+  const int col = job.z * 64 + (threadIdx.x & 7) * 8, row0 = job.y * 64 + (threadIdx.x >> 3);
+  float g[2][8], b[2][8];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int row = row0 + h * 32;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[h][j] = b[h][j] = 0.f;
+    if (row < m.rows && col < m.cols) {
+      row_load<T, 8>(in + (size_t)row * m.cols, col, m.cols, g[h]);
+      if (MOMENTUM) row_load<float, 8>(buf + (size_t)row * m.cols, col, m.cols, b[h]);
+    }
+  }
   double s = 0.0;
   for (int i = threadIdx.x; i < m.parts; i += 256) s += p.part[m.part + i];
 #pragma unroll
@@ -181,28 +198,14 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(NsArgs p) {
   lift = lift < 0 ? -lift : 0;
   if (job.y == 0 && job.z == 0 && threadIdx.x == 0) p.part[p.nparts + job.x] = (double)lift;
   const double scale = ldexp((double)m.scale / (norm + (double)p.eps), lift);
-  const T* in = (const T*)p.in + m.at;
-  const float* buf = MOMENTUM ? p.buf + m.at : nullptr;
-  const float gs = MOMENTUM ? p.hyper[1] : 1.f;
-  f16* x = p.ws + m.x;
-  const int col = job.z * 64 + (threadIdx.x & 7) * 8;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int row = job.y * 64 + h * 32 + (threadIdx.x >> 3);
-    float g[8], b[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) g[j] = 0.f;
-    if (row < m.rows && col < m.cols) {
-      row_load<T, 8>(in + (size_t)row * m.cols, col, m.cols, g);
-      if (MOMENTUM) {
-        row_load<float, 8>(buf + (size_t)row * m.cols, col, m.cols, b);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = ns_direction(g[j] * gs, b[j], p.mu, p.nesterov);
-      }
+    for (int j = 0; j < 8; ++j) {
+      if (MOMENTUM) g[h][j] = ns_direction(g[h][j] * gs, b[h][j], p.mu, p.nesterov);
+      g[h][j] = (float)((double)g[h][j] * scale);
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) g[j] = (float)((double)g[j] * scale);
-    ns_put(x + ns_at(m.cp, row, col), g);
+    ns_put(x + ns_at(m.cp, row0 + h * 32, col), g[h]);
   }
 }
 
@@ -398,14 +401,15 @@ __device__ __forceinline__ int ns_lift(const NsArgs& p, int mat, int k) {
 }
 
 // The fp32 tile in LDS, sums over all k, becomes the tile of A, or with POLY of B = b A + c A A, and its mirror image.
-template <int T, bool POLY>
-__device__ __forceinline__ void ns_symmetric_out(const NsArgs& p, const NsMat& m, int ti, int tj, int lift, float* tile) {
+// ROWS of its rows, from row `r0` of the tile on, are in LDS.
+template <int T, int ROWS, bool POLY>
+__device__ __forceinline__ void ns_symmetric_out(const NsArgs& p, const NsMat& m, int ti, int tj, int r0, int lift, float* tile) {
   f16* a = p.ws + m.a;
   f16* out = POLY ? a + (size_t)2 * m.mp * m.mp : a;
-  const int i0 = ti * T, j0 = tj * T;
+  const int i0 = ti * T + r0, j0 = tj * T;
   const float f = POLY ? ldexpf(NS_C / NS_GRAM_SCALE, -2 * lift) : NS_GRAM_SCALE / (m.scale * m.scale);
   // rows of the tile: eight consecutive columns a thread
-  for (int e = threadIdx.x; e < T * T / 8; e += 256) {
+  for (int e = threadIdx.x; e < ROWS * T / 8; e += 256) {
     const int r = e / (T / 8), c = e % (T / 8) * 8;
     const size_t at = ns_at(m.mp, i0 + r, j0 + c);
     float* t = tile + r * NS_PITCH(T) + c;
@@ -421,7 +425,7 @@ __device__ __forceinline__ void ns_symmetric_out(const NsArgs& p, const NsMat& m
   if (ti == tj) return;
   __syncthreads();
   // mirror image: consecutive lanes take consecutive columns of the tile in LDS, eight rows each
-  for (int e = threadIdx.x; e < T * T / 8; e += 256) {
+  for (int e = threadIdx.x; e < ROWS * T / 8; e += 256) {
     const int c = e % T, r = e / T * 8;
     float v[8];
 #pragma unroll
@@ -451,25 +455,33 @@ __device__ __forceinline__ void ns_symmetric(const NsArgs& p, const NsMat& m, co
       *(f32x4*)(slab + e * 4) = *(const f32x4*)(tile + e / (T / 4) * NS_PITCH(T) + e % (T / 4) * 4);
     return;
   }
-  ns_symmetric_out<T, POLY>(p, m, job.ti, job.tj, lift, tile);
+  ns_symmetric_out<T, T, POLY>(p, m, job.ti, job.tj, 0, lift, tile);
 }
 
-// Sums of the slabs of a tile, in order.
+// Sums of the slabs of a tile, in order; a workgroup takes 32 of its rows (the mean tile has few slabs of 64 KB, and one
+// workgroup would read them at the pace of its own loads).
+#define NS_JOIN_ROWS 32
 template <int T, bool POLY>
-__device__ __forceinline__ void ns_join_slabs(const NsArgs& p, const NsMat& m, const NsJob& job, int lift, char* smem) {
-  float* tile = (float*)smem;
-  const float* slab = p.slabs + (size_t)job.slab * 4096;
-  for (int e = threadIdx.x; e < T * T / 4; e += 256) {
-    f32x4 v = *(const f32x4*)(slab + e * 4);
-    for (int i = 1; i < job.k0; ++i) {
-      const f32x4 w = *(const f32x4*)(slab + (size_t)i * T * T + e * 4);
+__device__ __forceinline__ void ns_join_slabs(const NsArgs& p, const NsMat& m, const NsJob& job, int r0, int lift, float* tile) {
+  constexpr int N = NS_JOIN_ROWS * T / 4 / 256;
+  const float* slab = p.slabs + (size_t)job.slab * 4096 + r0 * T + threadIdx.x * 4;
+  f32x4 v[N];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] += w[j];
+  for (int n = 0; n < N; ++n) v[n] = *(const f32x4*)(slab + n * 1024);
+  for (int i = 1; i < job.k0; ++i)
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const f32x4 w = *(const f32x4*)(slab + (size_t)i * T * T + n * 1024);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[n][j] += w[j];
     }
-    *(f32x4*)(tile + e / (T / 4) * NS_PITCH(T) + e % (T / 4) * 4) = v;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int e = n * 256 + threadIdx.x;
+    *(f32x4*)(tile + e / (T / 4) * NS_PITCH(T) + e % (T / 4) * 4) = v[n];
   }
   __syncthreads();
-  ns_symmetric_out<T, POLY>(p, m, job.ti, job.tj, lift, tile);
+  ns_symmetric_out<T, NS_JOIN_ROWS, POLY>(p, m, job.ti, job.tj, r0, lift, tile);
 }
 
 enum { NS_NEXT = 0, NS_OUT = 1, NS_APPLY = 2 };
@@ -539,15 +551,17 @@ __global__ __launch_bounds__(256, 2) void ns_symmetric_kernel(NsArgs p, int k) {
 }
 
 template <bool POLY>
-__global__ __launch_bounds__(256, 2) void ns_join_kernel(NsArgs p, int k) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+__global__ __launch_bounds__(256) void ns_join_kernel(NsArgs p, int k) {
+  __shared__ __attribute__((aligned(16))) float tile[NS_JOIN_ROWS * NS_PITCH(128)];
   const NsJob job = (POLY ? p.poly_joins : p.gram_joins)[blockIdx.x];
+  const int r0 = blockIdx.y * NS_JOIN_ROWS;
+  if (r0 >= job.edge) return;
   const NsMat m = p.mats[job.mat];
   const int lift = POLY ? ns_lift(p, job.mat, k) : 0;
   if (job.edge == 128)
-    ns_join_slabs<128, POLY>(p, m, job, lift, smem);
+    ns_join_slabs<128, POLY>(p, m, job, r0, lift, tile);
   else
-    ns_join_slabs<64, POLY>(p, m, job, lift, smem);
+    ns_join_slabs<64, POLY>(p, m, job, r0, lift, tile);
 }
 
 template <int WHAT, typename O>
@@ -580,6 +594,12 @@ static int ns_tiles(int blocks, const NsArgs& a, int k, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
+template <bool POLY>
+static int ns_join(int tiles, const NsArgs& a, int k, hipStream_t st) {
+  hipLaunchKernelGGL((ns_join_kernel<POLY>), dim3(tiles, 128 / NS_JOIN_ROWS), dim3(256), 0, st, a, k);
+  return (int)hipGetLastError();
+}
+
 template <typename T>
 static int ns_first(const NsArgs& a, hipStream_t st) {
   if (a.buf != nullptr) {
@@ -603,9 +623,9 @@ extern "C" int dtfa_newton_schulz(const NsArgs* args, hipStream_t st) {
            : a.dtype == IO_F32 ? ns_first<float>(a, st) : -3;
   for (int k = 0; k < a.steps && rc == 0; ++k) {
     rc = ns_tiles<ns_symmetric_kernel<false>>(a.ngram, a, k, st);
-    if (rc == 0 && a.ngram_joins > 0) rc = ns_tiles<ns_join_kernel<false>>(a.ngram_joins, a, k, st);
+    if (rc == 0 && a.ngram_joins > 0) rc = ns_join<false>(a.ngram_joins, a, k, st);
     if (rc == 0) rc = ns_tiles<ns_symmetric_kernel<true>>(a.npoly, a, k, st);
-    if (rc == 0 && a.npoly_joins > 0) rc = ns_tiles<ns_join_kernel<true>>(a.npoly_joins, a, k, st);
+    if (rc == 0 && a.npoly_joins > 0) rc = ns_join<true>(a.npoly_joins, a, k, st);
     if (rc != 0) break;
     if (k + 1 < a.steps)
       rc = ns_tiles<ns_advance_kernel<NS_NEXT, float>>(a.nfull, a, k, st);

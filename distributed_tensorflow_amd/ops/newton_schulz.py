@@ -27,8 +27,8 @@ CHUNK = 8192              # elements per partial sum, at least
 # Measured on one MI355X, a CU's time in us: a tile job's fixed part (its first loads, the epilogue) and a k-step of 32.
 # A 128 x 128 tile does four times the work of a 64 x 64 tile in twice the time, so large tiles win once there are enough
 # of them for 256 CUs.
-JOB_US = {128: 4.0, 64: 2.0}
-STEP_US = {128: 0.72, 64: 0.36}
+JOB_US = {128: 7.0, 64: 2.5}
+STEP_US = {128: 0.72, 64: 0.33}
 CUS = 256
 SLOTS = 2 * CUS           # workgroups at a time
 MIN_STEPS = 8             # shortest piece of a cut reduction
@@ -85,12 +85,15 @@ def _up(v: int, edge: int) -> int:
     return -(-v // edge) * edge
 
 
-def _span(counts_costs) -> float:
-    """Time of a launch of (count, cost) jobs: an even share per CU plus what the last jobs, which are the short ones,
-    leave idle; never less than the longest job."""
-    total = sum(n * c for n, c in counts_costs)
-    longest = max(c for _, c in counts_costs)
-    return max(longest, total / CUS + 0.4 * longest)
+def _span(jobs: Sequence[Tuple[int, float]]) -> float:
+    """Time of a launch of (count, cost) jobs, longest first: an even share per CU (two workgroups share a CU's matrix
+    cores, so what counts is the work per CU), or what the CU with the most of the longest jobs takes."""
+    span = count = total = 0.0
+    for n, cost in sorted(jobs, key=lambda j: -j[1]):
+        count += n
+        total += n * cost
+        span = max(span, math.ceil(count / CUS) * cost)
+    return max(span, total / CUS * 1.08)
 
 
 def _choose(dims: Sequence[Tuple[int, int, int]], symmetric: bool) -> Tuple[int, int]:
@@ -99,15 +102,17 @@ def _choose(dims: Sequence[Tuple[int, int, int]], symmetric: bool) -> Tuple[int,
     best = (math.inf, 0, 0)
     for large_from in (128, 256, 512, 1024, 1 << 30):
         for piece in (1 << 30, 64, 32, 16, MIN_STEPS) if symmetric else (1 << 30,):
-            jobs, slabs = [], 0
+            jobs: Dict[float, int] = {}
+            slabs = 0
             for rows, cols, K in dims:
                 edge = 128 if min(rows, cols) >= large_from else 64
                 tr, tc, steps = -(-rows // edge), -(-cols // edge), _up(K, edge) // 32
                 n = tr * (tr + 1) // 2 if symmetric else tr * tc
                 cut = -(-steps // piece)
-                jobs.append((n * cut, _job_us(edge, -(-steps // cut))))
+                cost = _job_us(edge, -(-steps // cut))
+                jobs[cost] = jobs.get(cost, 0) + n * cut
                 slabs += n * cut * edge * edge * 4 if cut > 1 else 0
-            us = _span(jobs) + (5.0 + slabs * 2 / 3e6 if slabs else 0.0)
+            us = _span([(n, cost) for cost, n in jobs.items()]) + (4.0 + slabs * 2 / 3e6 if slabs else 0.0)
             if us < best[0]:
                 best = (us, large_from, piece)
     return best[1], best[2]
@@ -130,27 +135,43 @@ def _cut(jobs: np.ndarray, piece: int, slabs: int) -> Tuple[np.ndarray, np.ndarr
     return out, joins, slabs + len(out) * unit
 
 
+def _cut_tail(jobs: np.ndarray, slabs: int) -> Tuple[np.ndarray, np.ndarray, int]:
+    """Equal jobs beyond whole rounds of workgroups would run on a mostly idle card: their reductions are cut so that all
+    of it takes part."""
+    tail = len(jobs) % SLOTS
+    if len(jobs) < SLOTS or not 0 < tail <= SLOTS // 2:
+        return jobs, jobs[:0], slabs
+    steps = int(jobs[0, 5] - jobs[0, 4]) // 32
+    piece = max(MIN_STEPS, -(-steps // max(2, SLOTS // tail)))
+    cut, joins, slabs = _cut(jobs[-tail:], piece, slabs)
+    return np.concatenate([jobs[:-tail], cut]), joins, slabs
+
+
 def _over_xcds(groups: Sequence[np.ndarray]) -> np.ndarray:
-    """Workgroup n runs on XCD n % 8, each with its own L2: neighbouring tiles, which read the same rows, are dealt to the
-    XCDs in runs, longest jobs first, every run to the XCD with the least work so far; within an XCD the longest jobs
-    start first.  Shorter queues are filled up with empty jobs."""
-    total = sum(len(g) for g in groups)
-    run = max(1, min(32, total // 32))
-    runs = [g[at:at + run] for g in groups for at in range(0, len(g), run)]
+    """Workgroup n runs on XCD n % 8, each with its own L2: neighbouring tiles, which read the same rows, go to the same
+    XCD.  Every run of equal jobs is dealt out in eight consecutive parts, what does not divide job by job to the XCDs
+    with the least work so far; within an XCD the longest jobs start first.  Shorter queues end in empty jobs."""
+    runs = []
+    for g in groups:
+        runs += np.split(g, np.flatnonzero(np.diff(_cost(g))) + 1)
     runs.sort(key=lambda g: -float(_cost(g[:1])[0]))
     queues: List[List[np.ndarray]] = [[] for _ in range(8)]
-    load = [0.0] * 8
+    load = np.zeros(8)
     for g in runs:
-        x = load.index(min(load))
-        queues[x].append(g)
-        load[x] += float(_cost(g).sum())
+        each, cost = len(g) // 8, float(_cost(g[:1])[0])
+        for x in range(8):
+            queues[x].append(g[x * each:(x + 1) * each])
+        load += each * cost
+        for n in range(8 * each, len(g)):
+            x = int(np.argmin(load))
+            queues[x].append(g[n:n + 1])
+            load[x] += cost
     longest = max(sum(len(g) for g in q) for q in queues)
     out = np.zeros((longest, 8, 8), dtype=np.int32)
     out[:, :, 0] = -1
     for x, q in enumerate(queues):
-        if q:
-            jobs = np.concatenate(q)
-            out[:len(jobs), x] = jobs[np.argsort(-_cost(jobs), kind="stable")]
+        jobs = np.concatenate(q)
+        out[:len(jobs), x] = jobs[np.argsort(-_cost(jobs), kind="stable")]
     out = out.reshape(-1, 8)
     return out[:len(out) - int(np.argmax(out[::-1, 0] >= 0))]   # (no empty jobs behind the last)
 
@@ -186,10 +207,14 @@ class NsPlan:
             e = 128 if short >= gram_large else 64
             tiles = _jobs(k, *_tiles(mp // e, mp // e, lower=True), e, 0, max(rp, cp))
             jobs, joins, gram_slabs = _cut(tiles, gram_piece, gram_slabs)
+            if len(matrices) == 1 and not len(joins):
+                jobs, joins, gram_slabs = _cut_tail(jobs, gram_slabs)
             gram.append(jobs)
             gram_joins.append(joins)
             e = 128 if short >= poly_large else 64
             jobs, joins, poly_slabs = _cut(_jobs(k, *_tiles(mp // e, mp // e, lower=True), e, 0, mp), poly_piece, poly_slabs)
+            if len(matrices) == 1 and not len(joins):
+                jobs, joins, poly_slabs = _cut_tail(jobs, poly_slabs)
             poly.append(jobs)
             poly_joins.append(joins)
             e = 128 if short >= full_large else 64

@@ -113,6 +113,40 @@ def test_a_matrix_of_extremes_leaves_the_others_alone():
     assert got[1].isnan().all() and got[2].isnan().all() and not got[3].any()
 
 
+@pytest.mark.parametrize("rows,cols", [(300, 700), (700, 300), (130, 64), (256, 256)])
+@pytest.mark.parametrize("large_from,piece", [(128, 1), (128, 3), (1 << 30, 1), (1 << 30, 5), (128, 1 << 30), (1 << 30, 1 << 30)])
+def test_any_cut_of_the_work(monkeypatch, rows, cols, large_from, piece):
+    # tile edges and pieces that the estimate would not take at these sizes
+    monkeypatch.setattr(ns, "_choose", lambda dims, symmetric: (large_from, piece if symmetric else 1 << 30))
+    g = torch.stack([_matrix(rows, cols, torch.float32, 50 + s) for s in range(2)])
+    plan = ns.NsPlan([(0, rows, cols), (rows * cols, rows, cols)], g.device)
+    out = torch.empty_like(g)
+    plan.launch(inp=g, steps=5, out=out)
+    for o, m in zip(out, g):
+        _check(o, m)
+
+
+def test_leftover_tiles(monkeypatch):
+    # a whole round of workgroups and a few tiles more, whose reductions are cut
+    monkeypatch.setattr(ns, "_choose", lambda dims, symmetric: (1 << 30, 1 << 30))
+    monkeypatch.setattr(ns, "SLOTS", 16)
+    monkeypatch.setattr(ns, "MIN_STEPS", 1)
+    g = _matrix(380, 1000, torch.float32, 60)
+    plan = ns.NsPlan([(0, 380, 1000)], g.device)
+    assert plan.slabs > 0
+    out = torch.empty_like(g)
+    plan.launch(inp=g, steps=5, out=out)
+    _check(out, g)
+
+
+def test_large_matrix():
+    g = _matrix(4096, 4096, torch.float32, 61)
+    want = ref.newton_schulz(g.double(), 2)
+    base = (ref.newton_schulz(g, 2).double() - want).norm().item()
+    off = (F.orthogonalize(g, steps=2).double() - want).norm().item()
+    assert off <= (8 + math.sqrt(3 * 4096 / 16)) * base + 2.0 ** -23 * want.norm().item()
+
+
 def test_rank_one():
     u, v = _matrix(200, 1, torch.float32, 11), _matrix(1, 333, torch.float32, 12)
     g = (u @ v) * 1e6

@@ -63,7 +63,8 @@ def test_refusals():
 
 
 @pytest.mark.parametrize("shapes", [[(1, 1)], [(64, 64), (65, 64)], [(5, 700), (700, 5), (513, 2000), (1031, 600)],
-                                    [(2048, 512), (64, 64), (1000, 2048)]])
+                                    [(2048, 512), (64, 64), (1000, 2048)], [(4096, 4096)], [(4700, 3900)],
+                                    [(256, 2304)] * 6])
 def test_plan_covers_every_tile_once_and_stays_inside(shapes):
     places, at = [], 0
     for r, c in shapes:
