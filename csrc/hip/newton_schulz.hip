@@ -211,6 +211,9 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(NsArgs p) {
 
 // ---------------------------------------------------------------- products
 #define NS_BK 32
+#ifndef NS_STAGES128
+#define NS_STAGES128 2
+#endif
 
 // Tiles in LDS.  k contiguous: T rows of 128 bytes, 16-byte chunk plane * 4 + k / 8 at slot chunk ^ ns_swz(row): 16 rows
 // reading the same chunk touch every bank once.
@@ -240,7 +243,7 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
                                            f32x16 (&acc)[T / 64][T / 64]) {
   constexpr int OPER = T * NS_BK * 4;         // bytes of an operand's k-tile, both planes
   constexpr int STAGE = 2 * OPER;
-  constexpr int NST = T == 128 ? 2 : 4;
+  constexpr int NST = T == 128 ? NS_STAGES128 : 4;
   constexpr int LPS = OPER / 2048;            // LDS-DMA instructions per wave and k-tile
   constexpr int MT = T / 64;
   const int lane = threadIdx.x & 63;
@@ -272,12 +275,14 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
     step = 2 * NS_BK;
   }
   // (the swizzles repeat every 16 rows, or 4: every second instruction finds the same slots)
+  auto stage_one = [&](int buf, int i) {
+    glds16_untracked(src[i & 1] + (i >> 1) * pair, smem + buf * STAGE + wid * (OPER / 2) + i * 1024);
+    if (i == LPS - 2) src[0] += step;
+    if (i == LPS - 1) src[1] += step;
+  };
   auto stage = [&](int buf) {
-    char* dst = smem + buf * STAGE + wid * (OPER / 2);
 #pragma unroll
-    for (int i = 0; i < LPS; ++i) glds16_untracked(src[i & 1] + (i >> 1) * pair, dst + i * 1024);
-    src[0] += step;
-    src[1] += step;
+    for (int i = 0; i < LPS; ++i) stage_one(buf, i);
   };
 
   // fragments
@@ -300,35 +305,27 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
     return *(const f16x8*)(oper + row * 128 + (((lo * 4 + ks * 2 + (lane >> 5)) ^ ns_swz(row)) << 4));
   };
   f16x8 ph[2][MT], pl[2][MT], qh[2][MT], ql[2][MT];
-  auto load_frags = [&](int buf, int ks, int to) {
+  constexpr int FRAGS = 4 * MT;               // of a step of 16 k: Q hi, P hi, Q lo, P lo
+  auto load_frag = [&](int buf, int ks, int to, int i) {
     const char* at = smem + buf * STAGE;
-#pragma unroll
-    for (int u = 0; u < MT; ++u) {
-      ph[to][u] = frag(at, PK, wr * (T / 2) + u * 32, ks, 0);
-      qh[to][u] = frag(at + OPER, QK, wc * (T / 2) + u * 32, ks, 0);
-    }
-#pragma unroll
-    for (int u = 0; u < MT; ++u) {
-      ql[to][u] = frag(at + OPER, QK, wc * (T / 2) + u * 32, ks, 1);
-      pl[to][u] = frag(at, PK, wr * (T / 2) + u * 32, ks, 1);
-    }
+    const int u = i % MT;
+    if (i / MT == 0) qh[to][u] = frag(at + OPER, QK, wc * (T / 2) + u * 32, ks, 0);
+    if (i / MT == 1) ph[to][u] = frag(at, PK, wr * (T / 2) + u * 32, ks, 0);
+    if (i / MT == 2) ql[to][u] = frag(at + OPER, QK, wc * (T / 2) + u * 32, ks, 1);
+    if (i / MT == 3) pl[to][u] = frag(at, PK, wr * (T / 2) + u * 32, ks, 1);
   };
-  auto multiply = [&](int from) {
+  // the matrix instructions of a step of 16 k; `between` issues other work behind each, which runs in its shadow
+  auto multiply = [&](int from, auto between) {
 #pragma unroll
-    for (int u = 0; u < MT; ++u)
-#pragma unroll
-      for (int v = 0; v < MT; ++v)
-        acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[from][v], ph[from][u], acc[u][v], 0, 0, 0);
-#pragma unroll
-    for (int u = 0; u < MT; ++u)
-#pragma unroll
-      for (int v = 0; v < MT; ++v)
-        acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[from][v], ph[from][u], acc[u][v], 0, 0, 0);
-#pragma unroll
-    for (int u = 0; u < MT; ++u)
-#pragma unroll
-      for (int v = 0; v < MT; ++v)
-        acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[from][v], pl[from][u], acc[u][v], 0, 0, 0);
+    for (int n = 0; n < 3 * MT * MT; ++n) {
+      const int u = n / MT % MT, v = n % MT;
+      const f16x8 q = n / (MT * MT) == 1 ? ql[from][v] : qh[from][v];
+      const f16x8 w = n / (MT * MT) == 2 ? pl[from][u] : ph[from][u];
+      acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q, w, acc[u][v], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      between(n);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
 
 #pragma unroll
@@ -352,30 +349,48 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
   };
   arrive(0);
   if (NST - 1 < nk) stage(NST - 1);
-  load_frags(0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < FRAGS; ++i) load_frag(0, 0, 0, i);
   int cur = 0;
-  for (int kt = 0; kt < nk; ++kt) {
+  // Issued in a block, the eight LDS-DMA and eight LDS reads of a step would hold the wave for as long as its matrix
+  // instructions take; one behind each of these they cost next to nothing.
+  // (The last k-tile stands by itself: with one loop for all, the wait counts in front of the second group would have to
+  // hold for the pass without new reads as well, and wait for the new reads in all others.)
+  constexpr int N = 3 * MT * MT;
+  constexpr int RPM = (FRAGS + N - 1) / N;    // reads, and LDS-DMA, behind one matrix instruction
+  constexpr int SPM = (LPS + N - 1) / N;
+  for (int kt = 0; kt + 1 < nk; ++kt) {
     const int nxt = cur == NST - 1 ? 0 : cur + 1;
-    load_frags(cur, 1, 1);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(0);
-    __builtin_amdgcn_sched_barrier(0);
-    if (kt + 1 < nk) {
-      arrive(kt + 1);  // ... and k-tile kt has been read by every wave: its slot takes k-tile kt + NST
-      if (kt + NST < nk) stage(cur);
-      load_frags(nxt, 0, 0);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    multiply(1);
-    __builtin_amdgcn_sched_barrier(0);
+    multiply(0, [&](int n) {
+#pragma unroll
+      for (int i = n * RPM; i < n * RPM + RPM; ++i)
+        if (i < FRAGS) load_frag(cur, 1, 1, i);
+    });
+    arrive(kt + 1);  // ... and k-tile kt has been read by every wave: its slot takes k-tile kt + NST
+    const bool more = kt + NST < nk;
+    multiply(1, [&](int n) {
+#pragma unroll
+      for (int i = n * RPM; i < n * RPM + RPM; ++i)
+        if (i < FRAGS) load_frag(nxt, 0, 0, i);
+      if (more)
+#pragma unroll
+        for (int i = n * SPM; i < n * SPM + SPM; ++i)
+          if (i < LPS) stage_one(cur, i);
+    });
     cur = nxt;
   }
+  multiply(0, [&](int n) {
+#pragma unroll
+    for (int i = n * RPM; i < n * RPM + RPM; ++i)
+      if (i < FRAGS) load_frag(cur, 1, 1, i);
+  });
+  multiply(1, [](int) {});
 }
 
 // fp32 tile in LDS: 16-byte writes of 8 rows at a time hit every bank once at this pitch
 #define NS_PITCH(T) ((T) + 4)
-#define NS_LDS_BYTES (128 * NS_PITCH(128) * 4)
-static_assert(NS_LDS_BYTES >= 2 * 4 * 128 * NS_BK * 2 && NS_LDS_BYTES >= 4 * 4 * 64 * NS_BK * 2, "stages fit");
+#define NS_LDS_BYTES (NS_STAGES128 == 2 ? 128 * NS_PITCH(128) * 4 : NS_STAGES128 * 32768)
+static_assert(NS_LDS_BYTES >= NS_STAGES128 * 4 * 128 * NS_BK * 2 && NS_LDS_BYTES >= 4 * 4 * 64 * NS_BK * 2, "stages fit");
 
 // accumulators -> the tile [i][j] in LDS
 template <int T>
