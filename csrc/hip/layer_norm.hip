@@ -13,25 +13,33 @@
 //
 // A row belongs to TPR threads (a power of two, several rows to a wave below 64, a whole workgroup above), thread t
 // holding the NV vectors t, t + TPR, ... of 16 bytes.  Rows may start at any element (odd widths, channel slices):
-// gfx950 loads and stores 16 bytes at element alignment, and only the vector that crosses the end of a row goes element
-// by element.  Rows too long for the registers take the looping kernels at the end of the file.
+// gfx950 loads and stores 16 bytes at element alignment.  The elements behind the last whole vector, fewer than eight, are
+// one more scalar in each of the first threads (with an element-wise branch per vector instead, the compiler keeps every
+// vector's elements in registers of their own).  Rows too long for the registers take the looping kernels at the end of
+// the file.
 //
 // All arithmetic is fp32; outputs are rounded once.
 #include "row_io.h"
 
-// a per-column fp32 vector (gamma / beta), `fill` where there is none
-template <int VEC>
-__device__ __forceinline__ void ln_param(const float* __restrict__ p, int col, int C, float fill, float (&v)[VEC]) {
+// VEC values of a per-column fp32 vector (gamma / beta), `fill` where there is none; with TAIL those behind column C are 0
+template <int VEC, bool TAIL = false>
+__device__ __forceinline__ void ln_param(const float* __restrict__ p, int col, float fill, float (&v)[VEC], int C = 0) {
   if (p == nullptr) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) v[j] = fill;
-  } else {
+  } else if (TAIL) {
     row_load<float, VEC>(p, col, C, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 4) {
+      const RowVec<float>::V w = *(const RowVec<float>::V*)(p + col + j);
+      v[j] = w[0]; v[j + 1] = w[1]; v[j + 2] = w[2]; v[j + 3] = w[3];
+    }
   }
 }
 
-// Sum of N values per thread over the TPR threads of a row; every thread gets the sums.  Above one wave the waves'
-// sums meet in LDS (`red`, N * waves values): the caller's barrier discipline is two barriers a call.
+// Sum of N values per thread over the TPR threads of a row; every thread gets the sums.  Above one wave the sums of the
+// row's waves meet in LDS (`red`, N values for each wave of the workgroup); two barriers a call.
 template <int TPR, int N>
 __device__ __forceinline__ void ln_row_sum(float (&s)[N], float* red) {
 #pragma unroll
@@ -40,17 +48,17 @@ __device__ __forceinline__ void ln_row_sum(float (&s)[N], float* red) {
     for (int k = 0; k < N; ++k) s[k] += __shfl_xor(s[k], off, 64);
   if (TPR > 64) {
     constexpr int WAVES = TPR / 64;
-    const int wave = threadIdx.x >> 6;
+    const int wave = threadIdx.x >> 6, first = wave & ~(WAVES - 1);
     __syncthreads();  // the previous call's readers are done
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
-      for (int k = 0; k < N; ++k) red[k * WAVES + wave] = s[k];
+      for (int k = 0; k < N; ++k) red[wave * N + k] = s[k];
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       float t = 0.f;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) t += red[k * WAVES + w];
+      for (int w = 0; w < WAVES; ++w) t += red[(first + w) * N + k];
       s[k] = t;
     }
   }
@@ -71,11 +79,13 @@ struct LnFwd {
 
 template <typename T, int TPR, int NV>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(LnFwd p) {
+  typedef typename RowVec<T>::V V;
   constexpr int VEC = RowVec<T>::N;
   constexpr int BLOCK = TPR < 256 ? 256 : TPR;
   constexpr int RPB = BLOCK / TPR;  // rows side by side in a workgroup
-  __shared__ float red[TPR > 64 ? TPR / 64 : 1];
+  __shared__ float red[BLOCK / 64];
   const int t = threadIdx.x % TPR;
+  const int rest = p.cols % VEC, whole = p.cols - rest;  // the elements behind the last whole vector: one a thread
   const float n_c = (float)p.cols;  // (divided by, not multiplied with its inverse: the mean of equal values is that value)
   // (every thread of a wave takes part in the shuffles, and every thread of a workgroup in the barriers: the loop runs
   // by the workgroup's first row, rows past the end are computed from row 0 and not stored)
@@ -83,25 +93,33 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(L
     const long long row = base + threadIdx.x / TPR;
     const bool live = row < p.rows;
     const T* xr = (const T*)p.x + (live ? row : 0) * p.ldx;
-    float v[NV][VEC];
-    float s[1] = {0.f};
+    // held as stored and converted at each use: half the registers of fp32 copies, and it is resident waves that keep
+    // enough loads in flight
+    V v[NV];
+    float e = 0.f, s[1];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) row_load<T, VEC>(xr, (i * TPR + t) * VEC, p.cols, v[i]);
+    for (int i = 0; i < NV; ++i) {
+      const int col = (i * TPR + t) * VEC;
+      v[i] = V{};
+      if (col < whole) v[i] = *(const V*)(xr + col);
+    }
+    if (t < rest) e = (float)xr[whole + t];
+    s[0] = e;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) s[0] += v[i][j];
+      for (int j = 0; j < VEC; ++j) s[0] += (float)v[i][j];
     ln_row_sum<TPR, 1>(s, red);
     const float mean = s[0] / n_c;
-    s[0] = 0.f;
+    s[0] = t < rest ? (e - mean) * (e - mean) : 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      row_forget(v[i]);
+      float q = 0.f;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float d = v[i][j] - mean;
-        if ((i * TPR + t) * VEC + j < p.cols) s[0] += d * d;
-        v[i][j] = d;
-      }
+      for (int j = 0; j < VEC; ++j) q += ((float)v[i][j] - mean) * ((float)v[i][j] - mean);
+      s[0] += (i * TPR + t) * VEC < whole ? q : 0.f;
+    }
     ln_row_sum<TPR, 1>(s, red);
     const float rstd = 1.f / sqrtf(s[0] / n_c + p.eps);
     if (live) {
@@ -109,13 +127,21 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(L
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int col = (i * TPR + t) * VEC;
-        if (col >= p.cols) continue;
-        float g[VEC], b[VEC];
-        ln_param<VEC>(p.gamma, col, p.cols, 1.f, g);
-        ln_param<VEC>(p.beta, col, p.cols, 0.f, b);
+        __builtin_amdgcn_sched_barrier(0);  // one vector's gamma and beta at a time
+        row_forget(v[i]);
+        if (col < whole) {
+          float g[VEC], b[VEC];
+          ln_param<VEC>(p.gamma, col, 1.f, g);
+          ln_param<VEC>(p.beta, col, 0.f, b);
+          V o;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i][j] = v[i][j] * rstd * g[j] + b[j];
-        row_store<T, VEC>(yr, col, p.cols, v[i]);
+          for (int j = 0; j < VEC; ++j) o[j] = (T)(((float)v[i][j] - mean) * rstd * g[j] + b[j]);
+          *(V*)(yr + col) = o;
+        }
+      }
+      if (t < rest) {
+        const float g = p.gamma != nullptr ? p.gamma[whole + t] : 1.f, b = p.beta != nullptr ? p.beta[whole + t] : 0.f;
+        yr[whole + t] = (T)((e - mean) * rstd * g + b);
       }
       if (p.mean != nullptr && t == 0) {
         p.mean[row] = mean;
@@ -141,55 +167,83 @@ struct LnBwd {
 
 template <typename T, int TPR, int NV, bool PARAMS>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(LnBwd p) {
+  typedef typename RowVec<T>::V V;
   constexpr int VEC = RowVec<T>::N;
   constexpr int BLOCK = TPR < 256 ? 256 : TPR;
   constexpr int RPB = BLOCK / TPR;
-  __shared__ float red[TPR > 64 ? 2 * TPR / 64 : 1];
+  __shared__ float red[2 * BLOCK / 64];
   const int t = threadIdx.x % TPR;
-  const float n_c = (float)p.cols;  // (divided by, not multiplied with its inverse: the mean of equal values is that value)
-  float gam[NV][VEC], ag[NV][VEC], ab[NV][VEC];
+  const int rest = p.cols % VEC, whole = p.cols - rest;
+  const float n_c = (float)p.cols;
+  float gam[NV][VEC], ag[NV][VEC], ab[NV][VEC], game = 0.f, age = 0.f, abe = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int col = (i * TPR + t) * VEC;
-    if (col < p.cols) ln_param<VEC>(p.gamma, col, p.cols, 1.f, gam[i]);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      if (col >= p.cols) gam[i][j] = 0.f;
-      ag[i][j] = ab[i][j] = 0.f;
-    }
+    for (int j = 0; j < VEC; ++j) gam[i][j] = ag[i][j] = ab[i][j] = 0.f;
+    if (col < whole) ln_param<VEC>(p.gamma, col, 1.f, gam[i]);
   }
-  for (long long base = (long long)blockIdx.x * RPB; base < p.rows; base += (long long)gridDim.x * RPB) {
+  if (t < rest) game = p.gamma != nullptr ? p.gamma[whole + t] : 1.f;
+
+  // rows are fetched one ahead, held as stored
+  struct Row {
+    V x[NV], d[NV];
+    float xe, de, mean, rstd;
+  };
+  auto fetch = [&](long long base, Row& f) {
     const long long row = base + threadIdx.x / TPR;
-    const bool live = row < p.rows;
-    const long long at = live ? row : 0;
-    const T* xr = (const T*)p.x + at * p.ldx;
-    const T* gr = (const T*)p.dy + at * p.lddy;
-    float xh[NV][VEC], dy[NV][VEC];
+    const bool live = row < p.rows;  // (a row past the end is zeros and adds nothing)
+    const T* xr = (const T*)p.x + row * p.ldx;
+    const T* gr = (const T*)p.dy + row * p.lddy;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      row_load<T, VEC>(xr, (i * TPR + t) * VEC, p.cols, xh[i]);
-      row_load<T, VEC>(gr, (i * TPR + t) * VEC, p.cols, dy[i]);
+      const int col = (i * TPR + t) * VEC;
+      f.x[i] = f.d[i] = V{};
+      if (live && col < whole) {
+        f.x[i] = *(const V*)(xr + col);
+        f.d[i] = *(const V*)(gr + col);
+      }
     }
-    const float mean = p.mean[at], rstd = p.rstd[at];
-    float s[2] = {0.f, 0.f};
-    // (past the end of a row dy is zero, so these columns add nothing to any sum)
+    f.xe = f.de = f.mean = f.rstd = 0.f;
+    if (live) {
+      if (t < rest) {
+        f.xe = (float)xr[whole + t];
+        f.de = (float)gr[whole + t];
+      }
+      f.mean = p.mean[row];
+      f.rstd = p.rstd[row];
+    }
+  };
+  const long long stride = (long long)gridDim.x * RPB;
+  long long base = (long long)blockIdx.x * RPB;
+  Row r, next;
+  if (base < p.rows) fetch(base, r);
+  for (; base < p.rows; base += stride) {
+    const long long row = base + threadIdx.x / TPR;
+    const bool live = row < p.rows;
+    if (base + stride < p.rows) fetch(base + stride, next);
+    // (where there is no column dy is zero, so it adds nothing to any sum)
+    const float xhe = (r.xe - r.mean) * r.rstd;
+    float s[2] = {r.de * game, r.de * game * xhe};
+    if (PARAMS) {
+      age += r.de * xhe;
+      abe += r.de;
+    }
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      __builtin_amdgcn_sched_barrier(0);  // one vector at a time in fp32
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        xh[i][j] = (xh[i][j] - mean) * rstd;
-        const float d = dy[i][j] * gam[i][j];
+        const float xh = ((float)r.x[i][j] - r.mean) * r.rstd;
+        const float dy = (float)r.d[i][j];
+        const float d = dy * gam[i][j];
         s[0] += d;
-        s[1] += d * xh[i][j];
-      }
-    if (PARAMS && live) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          ag[i][j] += dy[i][j] * xh[i][j];
-          ab[i][j] += dy[i][j];
+        s[1] += d * xh;
+        if (PARAMS) {
+          ag[i][j] += dy * xh;
+          ab[i][j] += dy;
         }
+      }
     }
     if (p.dx != nullptr) {  // (uniform over the launch)
       ln_row_sum<TPR, 2>(s, red);
@@ -199,20 +253,30 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(L
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           const int col = (i * TPR + t) * VEC;
-          if (col >= p.cols) continue;
+          __builtin_amdgcn_sched_barrier(0);
+          row_forget(r.x[i]);
+          row_forget(r.d[i]);
+          if (col < whole) {
+            V o;
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) xh[i][j] = rstd * (dy[i][j] * gam[i][j] - m0 - xh[i][j] * m1);
-          row_store<T, VEC>(dr, col, p.cols, xh[i]);
+            for (int j = 0; j < VEC; ++j) {
+              const float xh = ((float)r.x[i][j] - r.mean) * r.rstd;
+              o[j] = (T)(r.rstd * ((float)r.d[i][j] * gam[i][j] - m0 - xh * m1));
+            }
+            *(V*)(dr + col) = o;
+          }
         }
+        if (t < rest) dr[whole + t] = (T)(r.rstd * (r.de * game - m0 - xhe * m1));
       }
     }
+    r = next;
   }
   if (!PARAMS) return;
   // threads of one column position in the rows side by side: lanes TPR apart, then the waves of the workgroup
   float* pg = p.part + (size_t)blockIdx.x * 2 * p.cols;
   float* pb = pg + p.cols;
 #pragma unroll
-  for (int off = 32; off >= TPR; off >>= 1)
+  for (int off = 32; off >= TPR; off >>= 1) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -220,34 +284,49 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(L
         ag[i][j] += __shfl_xor(ag[i][j], off, 64);
         ab[i][j] += __shfl_xor(ab[i][j], off, 64);
       }
-  constexpr bool WAVES_MEET = TPR <= 64;  // below that each wave holds other rows of the same columns
-  constexpr int CPW = (TPR < 64 ? TPR : 64) * VEC * NV;
-  __shared__ float meet[WAVES_MEET ? 4 : 1][WAVES_MEET ? CPW : 1];
-  if (WAVES_MEET) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    age += __shfl_xor(age, off, 64);
+    abe += __shfl_xor(abe, off, 64);
+  }
+  if (TPR <= 128) {  // several waves, or pairs of them, hold other rows of the same columns
+    constexpr int W = TPR;
+    constexpr int LEN = NV * VEC + 1, ROWS = TPR < 64 ? 4 : 256 / W;
+    __shared__ float meet[TPR <= 128 ? ROWS : 1][TPR <= 128 ? LEN * W : 1];
+    const int wave = threadIdx.x / (TPR < 64 ? 64 : W), lane = threadIdx.x % (TPR < 64 ? 64 : W);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       __syncthreads();
-      if (lane < TPR)
+      if (lane < W) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) meet[wave][(i * VEC + j) * (TPR < 64 ? TPR : 64) + t] = which ? ab[i][j] : ag[i][j];
+          for (int j = 0; j < VEC; ++j) meet[wave][(i * VEC + j) * W + t] = which ? ab[i][j] : ag[i][j];
+        meet[wave][NV * VEC * W + t] = which ? abe : age;
+      }
       __syncthreads();
-      for (int e = threadIdx.x; e < CPW; e += BLOCK) {
-        constexpr int W = TPR < 64 ? TPR : 64;
+      for (int e = threadIdx.x; e < LEN * W; e += BLOCK) {
         const int lt = e % W, ij = e / W;
-        const int col = ((ij / VEC) * TPR + lt) * VEC + ij % VEC;
-        if (col < p.cols) (which ? pb : pg)[col] = (meet[0][e] + meet[1][e]) + (meet[2][e] + meet[3][e]);
+        const bool tail = ij == NV * VEC;
+        const int col = tail ? whole + lt : ((ij / VEC) * TPR + lt) * VEC + ij % VEC;
+        if (col < (tail ? p.cols : whole)) {
+          float sum = meet[0][e];
+#pragma unroll
+          for (int w = 1; w < ROWS; ++w) sum += meet[w][e];
+          (which ? pb : pg)[col] = sum;
+        }
       }
     }
   } else {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * TPR + t) * VEC;
-      if (col >= p.cols) continue;
-      row_store<float, VEC>(pg, col, p.cols, ag[i]);
-      row_store<float, VEC>(pb, col, p.cols, ab[i]);
+      if (col < whole) {
+        row_store<float, VEC>(pg, col, p.cols, ag[i]);
+        row_store<float, VEC>(pb, col, p.cols, ab[i]);
+      }
+    }
+    if (t < rest) {
+      pg[whole + t] = age;
+      pb[whole + t] = abe;
     }
   }
 }
@@ -303,8 +382,8 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_long_kernel(LnFwd p) {
     for (long long c = threadIdx.x * VEC; c < p.cols; c += 1024 * VEC) {
       float g[VEC], b[VEC];
       row_load<T, VEC>(xr, (int)c, p.cols, v);
-      ln_param<VEC>(p.gamma, (int)c, p.cols, 1.f, g);
-      ln_param<VEC>(p.beta, (int)c, p.cols, 0.f, b);
+      ln_param<VEC, true>(p.gamma, (int)c, 1.f, g, p.cols);
+      ln_param<VEC, true>(p.beta, (int)c, 0.f, b, p.cols);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) v[j] = (v[j] - mean) * rstd * g[j] + b[j];
       row_store<T, VEC>(yr, (int)c, p.cols, v);
@@ -329,7 +408,7 @@ __global__ __launch_bounds__(1024) void layer_norm_dx_long_kernel(LnBwd p) {
     for (long long c = threadIdx.x * VEC; c < p.cols; c += 1024 * VEC) {
       row_load<T, VEC>(xr, (int)c, p.cols, x);
       row_load<T, VEC>(gr, (int)c, p.cols, d);
-      ln_param<VEC>(p.gamma, (int)c, p.cols, 1.f, g);
+      ln_param<VEC, true>(p.gamma, (int)c, 1.f, g, p.cols);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         s[0] += d[j] * g[j];
@@ -342,7 +421,7 @@ __global__ __launch_bounds__(1024) void layer_norm_dx_long_kernel(LnBwd p) {
     for (long long c = threadIdx.x * VEC; c < p.cols; c += 1024 * VEC) {
       row_load<T, VEC>(xr, (int)c, p.cols, x);
       row_load<T, VEC>(gr, (int)c, p.cols, d);
-      ln_param<VEC>(p.gamma, (int)c, p.cols, 1.f, g);
+      ln_param<VEC, true>(p.gamma, (int)c, 1.f, g, p.cols);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) x[j] = rstd * (d[j] * g[j] - m0 - ((x[j] - mean) * rstd) * m1);
       row_store<T, VEC>(dr, (int)c, p.cols, x);
@@ -405,11 +484,13 @@ static int ln_fwd(const LnFwd& p, long long nvec, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
+// `stats`: [2][rows] means and inverse standard deviations, or null.
 extern "C" int dtfa_layer_norm_fwd(const void* x, long long ldx, const float* gamma, const float* beta, void* y,
-                                   float* mean, float* rstd, long long rows, int cols, float eps, int dtype,
-                                   hipStream_t st) {
+                                   float* stats, long long rows, int cols, float eps, int dtype, hipStream_t st) {
   if (rows <= 0) return 0;
-  if (cols <= 0 || ldx < 0 || (mean == nullptr) != (rstd == nullptr)) return -1;
+  if (cols <= 0 || ldx < 0) return -1;
+  float* mean = stats;
+  float* rstd = stats != nullptr ? stats + rows : nullptr;
   const LnFwd p = {x, ldx, gamma, beta, y, mean, rstd, rows, cols, eps};
   const long long nvec = ln_vectors(cols, dtype);
   if (dtype == IO_BF16) return ln_fwd<bf16>(p, nvec, st);
@@ -422,12 +503,15 @@ extern "C" int dtfa_layer_norm_fwd(const void* x, long long ldx, const float* ga
 extern "C" int dtfa_layer_norm_bwd_parts(long long rows, int cols, int dtype) {
   const long long nvec = ln_vectors(cols, dtype);
   long long rpb = 1, most = 256;
-  if (nvec <= 256) {
+  if (nvec <= 128) {
     const int tpr = nvec <= 8 ? 8 : nvec <= 16 ? 16 : nvec <= 32 ? 32 : 64;
     rpb = 256 / tpr;
     most = 1024;
-  } else if (nvec <= 1024) {
+  } else if (nvec <= 512) {
+    rpb = nvec <= 256 ? 2 : 1;
     most = 768;
+  } else if (nvec <= 1024) {
+    most = 512;
   } else if (nvec > 2048) {  // column strips of the long form
     const long long strips = (nvec + 255) / 256;
     most = strips >= 1024 ? 1 : 1024 / strips;
@@ -453,9 +537,9 @@ static int ln_bwd(const LnBwd& p, long long nvec, int parts, hipStream_t st) {
   if (nvec <= 32) return ln_bwd_launch<T, 32, 1>(p, parts, st);
   if (nvec <= 64) return ln_bwd_launch<T, 64, 1>(p, parts, st);
   if (nvec <= 128) return ln_bwd_launch<T, 64, 2>(p, parts, st);
-  if (nvec <= 256) return ln_bwd_launch<T, 64, 4>(p, parts, st);
+  if (nvec <= 256) return ln_bwd_launch<T, 128, 2>(p, parts, st);
   if (nvec <= 512) return ln_bwd_launch<T, 256, 2>(p, parts, st);
-  if (nvec <= 1024) return ln_bwd_launch<T, 256, 4>(p, parts, st);
+  if (nvec <= 1024) return ln_bwd_launch<T, 512, 2>(p, parts, st);
   if (nvec <= 2048) return ln_bwd_launch<T, 512, 4>(p, parts, st);
   if (p.dx != nullptr) {
     const long long grid = p.rows < LN_MAX_GRID ? p.rows : LN_MAX_GRID;
@@ -470,12 +554,12 @@ static int ln_bwd(const LnBwd& p, long long nvec, int parts, hipStream_t st) {
 
 // `part`: [dtfa_layer_norm_bwd_parts()][2][cols] fp32 scratch, null when neither dgamma nor dbeta is wanted.
 extern "C" int dtfa_layer_norm_bwd(const void* x, long long ldx, const void* dy, long long lddy, const float* gamma,
-                                   const float* mean, const float* rstd, void* dx, float* part, float* dgamma,
-                                   float* dbeta, long long rows, int cols, int dtype, hipStream_t st) {
+                                   const float* stats, void* dx, float* part, float* dgamma, float* dbeta, long long rows,
+                                   int cols, int dtype, hipStream_t st) {
   if (cols <= 0 || rows <= 0 || ldx < 0 || lddy < 0) return -1;
   if ((dgamma != nullptr || dbeta != nullptr) != (part != nullptr)) return -1;
   if (dx == nullptr && part == nullptr) return 0;
-  const LnBwd p = {x, ldx, dy, lddy, gamma, mean, rstd, dx, part, rows, cols};
+  const LnBwd p = {x, ldx, dy, lddy, gamma, stats, stats + rows, dx, part, rows, cols};
   const long long nvec = ln_vectors(cols, dtype);
   const int parts = dtfa_layer_norm_bwd_parts(rows, cols, dtype);
   int rc = dtype == IO_BF16 ? ln_bwd<bf16>(p, nvec, parts, st)

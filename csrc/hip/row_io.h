@@ -13,6 +13,16 @@ struct RowVec {
   typedef T V __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
 
+// The compiler would convert a vector once and keep the fp32 copies; after this it converts again.
+template <typename V>
+__device__ __forceinline__ void row_forget(V& v) {
+  typedef unsigned U __attribute__((ext_vector_type(4)));
+  static_assert(sizeof(V) == sizeof(U), "16 bytes");
+  U u = __builtin_bit_cast(U, v);
+  asm volatile("" : "+v"(u));
+  v = __builtin_bit_cast(V, u);
+}
+
 // VEC (a multiple of the 16-byte vector) consecutive elements from column `col` of a row of C as fp32; zeros behind
 // the end
 template <typename T, int VEC>

@@ -1033,17 +1033,17 @@ def global_avg_pool(x):
 class _LayerNormFn(Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, eps, params):
-        y, mean, rstd = K.layer_norm_fwd(x, gamma, beta, eps, want_stats=True)
+        y, stats = K.layer_norm_fwd(x, gamma, beta, eps, want_stats=True)
         ctx.params = params
-        ctx.save_for_backward(x, gamma, mean, rstd)
+        ctx.save_for_backward(x, gamma, stats)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, gamma, mean, rstd = ctx.saved_tensors
+        x, gamma, stats = ctx.saved_tensors
         want_dx, want_dg, want_db = ctx.needs_input_grad[:3]
-        dx, dg, db = K.layer_norm_bwd(dy, x, gamma, mean, rstd, want_dx, want_dg, want_db)
+        dx, dg, db = K.layer_norm_bwd(dy, x, gamma, stats, want_dx, want_dg, want_db)
         pg, pb = ctx.params
         return dx, _deliver_small(pg, dg), _deliver_small(pb, db), None, None
 

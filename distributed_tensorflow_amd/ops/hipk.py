@@ -136,10 +136,10 @@ class _Sigs:
     dtfa_act_l2_bwd = [c_void, c_void, c_void, c_float, c_void, c_ll, c_void]
     dtfa_adam = [c_void, c_void, c_void, c_void, c_int, c_void, c_ll, c_void, c_float, c_float, c_float, c_void]
     dtfa_momentum = [c_void, c_void, c_void, c_int, c_void, c_ll, c_void, c_float, c_float, c_int, c_void]
-    dtfa_layer_norm_fwd = [c_void, c_ll, c_void, c_void, c_void, c_void, c_void, c_ll, c_int, c_float, c_int, c_void]
+    dtfa_layer_norm_fwd = [c_void, c_ll, c_void, c_void, c_void, c_void, c_ll, c_int, c_float, c_int, c_void]
     dtfa_layer_norm_bwd_parts = [c_ll, c_int, c_int]
-    dtfa_layer_norm_bwd = [c_void, c_ll, c_void, c_ll, c_void, c_void, c_void, c_void, c_void, c_void, c_void, c_ll, c_int,
-                           c_int, c_void]
+    dtfa_layer_norm_bwd = [c_void, c_ll, c_void, c_ll, c_void, c_void, c_void, c_void, c_void, c_void, c_ll, c_int, c_int,
+                           c_void]
     dtfa_newton_schulz = [c_void, c_void]
     dtfa_cast_f32_bf16 = [c_void, c_void, c_ll, c_void]
     dtfa_mask_mul = [c_void, c_void, c_void, c_ll, c_void]
@@ -156,7 +156,8 @@ class _Sigs:
 
 
 def stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # (the raw handle: building a torch.cuda.Stream object around it costs more than the rest of a launch's host work)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 _same_device = contextlib.nullcontext()

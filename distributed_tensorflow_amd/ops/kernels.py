@@ -574,26 +574,24 @@ def _ln_check(x: torch.Tensor, gamma, beta) -> None:
 def layer_norm_fwd(x: torch.Tensor, gamma: Optional[torch.Tensor], beta: Optional[torch.Tensor], eps: float,
                    want_stats: bool = False):
     """``(x - mean) / sqrt(var + eps) * gamma + beta`` over the last axis, in ``x``'s dtype and contiguous.  ``x``: bf16,
-    fp16 or fp32, contiguous or a channel slice.  Returns ``(y, mean, rstd)``, the statistics one fp32 value a row (None
-    unless ``want_stats``)."""
+    fp16 or fp32, contiguous or a channel slice.  Returns ``(y, stats)``, ``stats`` = fp32 ``[2, rows]`` of means and inverse
+    standard deviations, what :func:`layer_norm_bwd` wants (None unless ``want_stats``)."""
     _ln_check(x, gamma, beta)
     cols = x.shape[-1]
     rows = x.numel() // cols
     with hipk.device_of(x):
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        mean = rstd = None
-        if want_stats:
-            mean, rstd = torch.empty((2, rows), dtype=F32, device=x.device).unbind(0)
+        stats = torch.empty((2, rows), dtype=F32, device=x.device) if want_stats else None
         if rows:
             xr, ldx = _ln_rows(x)
             hipk.check(hipk.lib().dtfa_layer_norm_fwd(xr.data_ptr(), ldx, hipk.ptr(gamma), hipk.ptr(beta), y.data_ptr(),
-                                                      hipk.ptr(mean), hipk.ptr(rstd), rows, cols, float(eps),
-                                                      _LN_DTYPES[x.dtype], hipk.stream()), "layer_norm_fwd")
-    return y, mean, rstd
+                                                      hipk.ptr(stats), rows, cols, float(eps), _LN_DTYPES[x.dtype],
+                                                      hipk.stream()), "layer_norm_fwd")
+    return y, stats
 
 
-def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, gamma: Optional[torch.Tensor], mean: torch.Tensor,
-                   rstd: torch.Tensor, want_dx: bool = True, want_dgamma: bool = True, want_dbeta: bool = True):
+def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, gamma: Optional[torch.Tensor], stats: torch.Tensor,
+                   want_dx: bool = True, want_dgamma: bool = True, want_dbeta: bool = True):
     """Gradients ``(dx, dgamma, dbeta)`` of :func:`layer_norm_fwd`, None where not wanted.  ``dgamma`` / ``dbeta`` (fp32)
     are summed in a fixed order."""
     _ln_check(x, gamma, None)
@@ -602,10 +600,10 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, gamma: Optional[torch.Tens
                          % (tuple(dy.shape), dy.dtype, tuple(x.shape), x.dtype))
     cols = x.shape[-1]
     rows = x.numel() // cols
-    for t, nm in ((mean, "mean"), (rstd, "rstd")):
-        hipk.require(t, F32, "layer_norm: " + nm)
-        if t.numel() != rows or t.device != x.device:
-            raise ValueError("layer_norm backward: %s must have one value for each of %d rows" % (nm, rows))
+    hipk.require(stats, F32, "layer_norm: stats")
+    if stats.shape != (2, rows) or stats.device != x.device:
+        raise ValueError("layer_norm backward: stats must be two values for each of %d rows, got shape %s"
+                         % (rows, tuple(stats.shape)))
     with hipk.device_of(x):
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
         fresh = torch.empty if rows else torch.zeros
@@ -617,9 +615,8 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, gamma: Optional[torch.Tens
             part = None
             if want_dgamma or want_dbeta:
                 part = torch.empty((L.dtfa_layer_norm_bwd_parts(rows, cols, dt), 2, cols), dtype=F32, device=x.device)
-            hipk.check(L.dtfa_layer_norm_bwd(xr.data_ptr(), ldx, gr.data_ptr(), ldg, hipk.ptr(gamma), mean.data_ptr(),
-                                             rstd.data_ptr(), hipk.ptr(dx), hipk.ptr(part), hipk.ptr(dgamma),
-                                             hipk.ptr(dbeta), rows, cols, dt, hipk.stream()), "layer_norm_bwd")
+            hipk.check(L.dtfa_layer_norm_bwd(xr.data_ptr(), ldx, gr.data_ptr(), ldg, hipk.ptr(gamma), stats.data_ptr(),
+                                             hipk.ptr(dx), hipk.ptr(part), hipk.ptr(dgamma), hipk.ptr(dbeta), rows, cols, dt, hipk.stream()), "layer_norm_bwd")
     return dx, dgamma, dbeta
 
 

@@ -28,7 +28,7 @@ CHUNK = 8192              # elements per partial sum, at least
 # A 128 x 128 tile does four times the work of a 64 x 64 tile in twice the time, so large tiles win once there are enough
 # of them for 256 CUs.
 JOB_US = {128: 7.0, 64: 2.5}
-STEP_US = {128: 0.72, 64: 0.33}
+STEP_US = {128: 0.66, 64: 0.31}
 CUS = 256
 SLOTS = 2 * CUS           # workgroups at a time
 MIN_STEPS = 8             # shortest piece of a cut reduction
@@ -101,7 +101,7 @@ def _choose(dims: Sequence[Tuple[int, int, int]], symmetric: bool) -> Tuple[int,
     stage whose outputs are ``rows x cols`` sums over ``K`` for (rows, cols, K) in ``dims``."""
     best = (math.inf, 0, 0)
     for large_from in (128, 256, 512, 1024, 1 << 30):
-        for piece in (1 << 30, 64, 32, 16, MIN_STEPS) if symmetric else (1 << 30,):
+        for piece in (1 << 30, 64, 48, 32, 24, 16, MIN_STEPS) if symmetric else (1 << 30,):
             jobs: Dict[float, int] = {}
             slabs = 0
             for rows, cols, K in dims:

@@ -95,8 +95,8 @@ def test_forward_and_gradients(rows, cols, dtype):
 def test_channel_slices_need_no_copy(rows, cols, pitch, dtype):
     x, dy, gamma, beta = _inputs(rows, cols, dtype, pitch, pitch)
     assert not x.is_contiguous() and K._ln_rows(x)[0] is x
-    y, mean, rstd = K.layer_norm_fwd(x, gamma, beta, 1e-3, want_stats=True)
-    grads = K.layer_norm_bwd(dy, x, gamma, mean, rstd)
+    y, stats = K.layer_norm_fwd(x, gamma, beta, 1e-3, want_stats=True)
+    grads = K.layer_norm_bwd(dy, x, gamma, stats)
     want, err = _exact(x, gamma, beta, dy, 1e-3)
     for got, w, e, name in zip((y,) + grads, want, err, ("y", "dx", "dgamma", "dbeta")):
         _check(got, w, e, name)
@@ -137,10 +137,10 @@ def test_without_scale_or_offset(with_gamma, with_beta):
 
 def test_gradients_only_where_wanted():
     x, dy, gamma, beta = _inputs(50, 2304, torch.bfloat16, 6)
-    _, mean, rstd = K.layer_norm_fwd(x, gamma, beta, 1e-5, want_stats=True)
-    full = K.layer_norm_bwd(dy, x, gamma, mean, rstd)
+    _, stats = K.layer_norm_fwd(x, gamma, beta, 1e-5, want_stats=True)
+    full = K.layer_norm_bwd(dy, x, gamma, stats)
     for want in [(True, False, False), (False, True, False), (False, False, True), (False, True, True), (False, False, False)]:
-        for w, t, f in zip(want, K.layer_norm_bwd(dy, x, gamma, mean, rstd, *want), full):
+        for w, t, f in zip(want, K.layer_norm_bwd(dy, x, gamma, stats, *want), full):
             assert (t is None) if not w else torch.equal(t, f)
 
 
@@ -172,12 +172,12 @@ def test_broadcast_upstream_gradient():
 def test_rows_of_extremes_do_not_touch_their_neighbours():
     x, dy, gamma, beta = _inputs(40, 136, torch.float32, 9)
     clean = K.layer_norm_fwd(x, gamma, beta, 1e-5, want_stats=True)
-    dx = K.layer_norm_bwd(dy, x, gamma, clean[1], clean[2])[0]
+    dx = K.layer_norm_bwd(dy, x, gamma, clean[1])[0]
     bad = x.clone()
     bad[3, 5], bad[4, 0], bad[5, 135] = float("nan"), float("inf"), float("-inf")
     bad[6] = torch.finfo(torch.float32).min
-    y, mean, rstd = K.layer_norm_fwd(bad, gamma, beta, 1e-5, want_stats=True)
-    dxb = K.layer_norm_bwd(dy, bad, gamma, mean, rstd)[0]
+    y, stats = K.layer_norm_fwd(bad, gamma, beta, 1e-5, want_stats=True)
+    dxb = K.layer_norm_bwd(dy, bad, gamma, stats)[0]
     rest = [i for i in range(40) if i not in (3, 4, 5, 6)]
     assert torch.equal(y[rest], clean[0][rest]) and torch.equal(dxb[rest], dx[rest])
     assert y[3:6].isnan().all() and not y[rest].isnan().any()
@@ -204,10 +204,10 @@ def test_no_rows():
 
 def test_repeatable():
     x, dy, gamma, beta = _inputs(20000, 64, torch.bfloat16, 12)
-    _, mean, rstd = K.layer_norm_fwd(x, gamma, beta, 1e-5, want_stats=True)
-    first = K.layer_norm_bwd(dy, x, gamma, mean, rstd)
+    _, stats = K.layer_norm_fwd(x, gamma, beta, 1e-5, want_stats=True)
+    first = K.layer_norm_bwd(dy, x, gamma, stats)
     for _ in range(3):
-        assert all(torch.equal(a, b) for a, b in zip(first, K.layer_norm_bwd(dy, x, gamma, mean, rstd)))
+        assert all(torch.equal(a, b) for a, b in zip(first, K.layer_norm_bwd(dy, x, gamma, stats)))
 
 
 def test_more_than_2_to_31_elements():
@@ -218,8 +218,8 @@ def test_more_than_2_to_31_elements():
     dy = torch.zeros_like(x)
     dy[-2:] = 0.25
     gamma = torch.randn(cols, generator=gen, device="cuda")
-    y, mean, rstd = K.layer_norm_fwd(x, gamma, None, 1e-5, want_stats=True)
-    dx, dg, db = K.layer_norm_bwd(dy, x, gamma, mean, rstd)
+    y, stats = K.layer_norm_fwd(x, gamma, None, 1e-5, want_stats=True)
+    dx, dg, db = K.layer_norm_bwd(dy, x, gamma, stats)
     want, err = _exact(x[-3:], gamma, None, dy[-3:], 1e-5)
     for got, w, e, name in zip((y[-3:], dx[-3:], dg, db), want, err, ("y", "dx", "dgamma", "dbeta")):
         _check(got, w, e, name)
@@ -231,8 +231,8 @@ def test_captured_forward_and_backward_replays():
     fresh = [_inputs(300, 520, torch.bfloat16, 20 + i)[:2] for i in range(3)]
 
     def once():
-        y, mean, rstd = K.layer_norm_fwd(x, gamma, beta, 1e-5, want_stats=True)
-        return (y,) + K.layer_norm_bwd(dy, x, gamma, mean, rstd)
+        y, stats = K.layer_norm_fwd(x, gamma, beta, 1e-5, want_stats=True)
+        return (y,) + K.layer_norm_bwd(dy, x, gamma, stats)
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -286,9 +286,9 @@ def test_refusals():
                 lambda: F.layer_norm(x, v.bfloat16(), v), lambda: F.layer_norm(x, v[:63], v),
                 lambda: F.layer_norm(x, v, v.view(8, 8)), lambda: F.layer_norm(x, v.cpu(), v),
                 lambda: F.layer_norm(x[:, :0]), lambda: F.layer_norm(x, torch.ones(128, device="cuda")[::2], v),
-                lambda: K.layer_norm_bwd(x.bfloat16(), x, v, x[:, 0].contiguous(), x[:, 0].contiguous()),
-                lambda: K.layer_norm_bwd(x[:3], x, v, x[:, 0].contiguous(), x[:, 0].contiguous()),
-                lambda: K.layer_norm_bwd(x, x, v, v, v), lambda: K.layer_norm_fwd(x.cpu(), None, None, 1e-5)]:
+                lambda: K.layer_norm_bwd(x.bfloat16(), x, v, torch.zeros(2, 4, device="cuda")),
+                lambda: K.layer_norm_bwd(x[:3], x, v, torch.zeros(2, 4, device="cuda")),
+                lambda: K.layer_norm_bwd(x, x, v, torch.zeros(2, 3, device="cuda")), lambda: K.layer_norm_fwd(x.cpu(), None, None, 1e-5)]:
         with pytest.raises(ValueError):
             bad()
     xg = x.clone().requires_grad_(True)
