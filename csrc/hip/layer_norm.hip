@@ -38,6 +38,14 @@ __device__ __forceinline__ void ln_param(const float* __restrict__ p, int col, f
   }
 }
 
+// A thread's row among those side by side in its workgroup.  From one wave on it is the same for the whole wave, and said
+// to be: the rows' addresses then live in scalar registers.
+template <int TPR, int BLOCK>
+__device__ __forceinline__ int ln_row_of_thread() {
+  if (TPR == BLOCK) return 0;
+  return TPR >= 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TPR) : threadIdx.x / TPR;
+}
+
 // Sum of N values per thread over the TPR threads of a row; every thread gets the sums.  Above one wave the sums of the
 // row's waves meet in LDS (`red`, N values for each wave of the workgroup); two barriers a call.
 template <int TPR, int N>
@@ -90,25 +98,25 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(L
   // (every thread of a wave takes part in the shuffles, and every thread of a workgroup in the barriers: the loop runs
   // by the workgroup's first row, rows past the end are computed from row 0 and not stored)
   for (long long base = (long long)blockIdx.x * RPB; base < p.rows; base += (long long)gridDim.x * RPB) {
-    const long long row = base + threadIdx.x / TPR;
+    const long long row = base + ln_row_of_thread<TPR, BLOCK>();
     const bool live = row < p.rows;
     const T* xr = (const T*)p.x + (live ? row : 0) * p.ldx;
     // held as stored and converted at each use: half the registers of fp32 copies, and it is resident waves that keep
     // enough loads in flight
-    V v[NV];
+    row_u32x4 v[NV];
     float e = 0.f, s[1];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * TPR + t) * VEC;
-      v[i] = V{};
-      if (col < whole) v[i] = *(const V*)(xr + col);
+      v[i] = row_u32x4{0, 0, 0, 0};
+      if (col < whole) v[i] = row_raw<T>(xr + col);
     }
     if (t < rest) e = (float)xr[whole + t];
     s[0] = e;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) s[0] += (float)v[i][j];
+      for (int j = 0; j < VEC; ++j) s[0] += row_element<T>(v[i], j);
     ln_row_sum<TPR, 1>(s, red);
     const float mean = s[0] / n_c;
     s[0] = t < rest ? (e - mean) * (e - mean) : 0.f;
@@ -117,7 +125,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(L
       row_forget(v[i]);
       float q = 0.f;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) q += ((float)v[i][j] - mean) * ((float)v[i][j] - mean);
+      for (int j = 0; j < VEC; ++j) q += (row_element<T>(v[i], j) - mean) * (row_element<T>(v[i], j) - mean);
       s[0] += (i * TPR + t) * VEC < whole ? q : 0.f;
     }
     ln_row_sum<TPR, 1>(s, red);
@@ -135,7 +143,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(L
           ln_param<VEC>(p.beta, col, 0.f, b);
           V o;
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) o[j] = (T)(((float)v[i][j] - mean) * rstd * g[j] + b[j]);
+          for (int j = 0; j < VEC; ++j) o[j] = (T)((row_element<T>(v[i], j) - mean) * rstd * g[j] + b[j]);
           *(V*)(yr + col) = o;
         }
       }
@@ -166,7 +174,7 @@ struct LnBwd {
 };
 
 template <typename T, int TPR, int NV, bool PARAMS>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(LnBwd p) {
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV == 1 ? 4 : NV == 2 ? 3 : 2) void layer_norm_bwd_kernel(LnBwd p) {
   typedef typename RowVec<T>::V V;
   constexpr int VEC = RowVec<T>::N;
   constexpr int BLOCK = TPR < 256 ? 256 : TPR;
@@ -175,33 +183,45 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(L
   const int t = threadIdx.x % TPR;
   const int rest = p.cols % VEC, whole = p.cols - rest;
   const float n_c = (float)p.cols;
-  float gam[NV][VEC], ag[NV][VEC], ab[NV][VEC], game = 0.f, age = 0.f, abe = 0.f;
+  float ag[NV][VEC], ab[NV][VEC], game = 0.f, age = 0.f, abe = 0.f;
+  // a thread's gamma waits in LDS, in a place of its own: the registers go to the rows in flight
+  __shared__ f32x4 gamma_lds[NV * VEC / 4][BLOCK];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int col = (i * TPR + t) * VEC;
+    float g[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) gam[i][j] = ag[i][j] = ab[i][j] = 0.f;
-    if (col < whole) ln_param<VEC>(p.gamma, col, 1.f, gam[i]);
+    for (int j = 0; j < VEC; ++j) g[j] = ag[i][j] = ab[i][j] = 0.f;
+    if (col < whole) ln_param<VEC>(p.gamma, col, 1.f, g);
+#pragma unroll
+    for (int j = 0; j < VEC; j += 4) gamma_lds[(i * VEC + j) / 4][threadIdx.x] = f32x4{g[j], g[j + 1], g[j + 2], g[j + 3]};
   }
+  auto gamma_of = [&](int i, float (&g)[VEC]) {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 4) {
+      const f32x4 w = gamma_lds[(i * VEC + j) / 4][threadIdx.x];
+      g[j] = w[0]; g[j + 1] = w[1]; g[j + 2] = w[2]; g[j + 3] = w[3];
+    }
+  };
   if (t < rest) game = p.gamma != nullptr ? p.gamma[whole + t] : 1.f;
 
   // rows are fetched one ahead, held as stored
   struct Row {
-    V x[NV], d[NV];
+    row_u32x4 x[NV], d[NV];
     float xe, de, mean, rstd;
   };
   auto fetch = [&](long long base, Row& f) {
-    const long long row = base + threadIdx.x / TPR;
+    const long long row = base + ln_row_of_thread<TPR, BLOCK>();
     const bool live = row < p.rows;  // (a row past the end is zeros and adds nothing)
     const T* xr = (const T*)p.x + row * p.ldx;
     const T* gr = (const T*)p.dy + row * p.lddy;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * TPR + t) * VEC;
-      f.x[i] = f.d[i] = V{};
+      f.x[i] = f.d[i] = row_u32x4{0, 0, 0, 0};
       if (live && col < whole) {
-        f.x[i] = *(const V*)(xr + col);
-        f.d[i] = *(const V*)(gr + col);
+        f.x[i] = row_raw<T>(xr + col);
+        f.d[i] = row_raw<T>(gr + col);
       }
     }
     f.xe = f.de = f.mean = f.rstd = 0.f;
@@ -219,7 +239,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(L
   Row r, next;
   if (base < p.rows) fetch(base, r);
   for (; base < p.rows; base += stride) {
-    const long long row = base + threadIdx.x / TPR;
+    const long long row = base + ln_row_of_thread<TPR, BLOCK>();
     const bool live = row < p.rows;
     if (base + stride < p.rows) fetch(base + stride, next);
     // (where there is no column dy is zero, so it adds nothing to any sum)
@@ -232,11 +252,13 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(L
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       __builtin_amdgcn_sched_barrier(0);  // one vector at a time in fp32
+      float gam[VEC];
+      gamma_of(i, gam);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float xh = ((float)r.x[i][j] - r.mean) * r.rstd;
-        const float dy = (float)r.d[i][j];
-        const float d = dy * gam[i][j];
+        const float xh = (row_element<T>(r.x[i], j) - r.mean) * r.rstd;
+        const float dy = row_element<T>(r.d[i], j);
+        const float d = dy * gam[j];
         s[0] += d;
         s[1] += d * xh;
         if (PARAMS) {
@@ -244,6 +266,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(L
           ab[i][j] += dy;
         }
       }
+      // (else these sums sink into the branch below, and every xhat and dy stays in registers until then)
+      asm volatile("" : "+v"(s[0]), "+v"(s[1]));
     }
     if (p.dx != nullptr) {  // (uniform over the launch)
       ln_row_sum<TPR, 2>(s, red);
@@ -258,10 +282,12 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(L
           row_forget(r.d[i]);
           if (col < whole) {
             V o;
+            float gam[VEC];
+            gamma_of(i, gam);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-              const float xh = ((float)r.x[i][j] - r.mean) * r.rstd;
-              o[j] = (T)(r.rstd * ((float)r.d[i][j] * gam[i][j] - m0 - xh * m1));
+              const float xh = (row_element<T>(r.x[i], j) - r.mean) * r.rstd;
+              o[j] = (T)(r.rstd * (row_element<T>(r.d[i], j) * gam[j] - m0 - xh * m1));
             }
             *(V*)(dr + col) = o;
           }
@@ -502,17 +528,10 @@ extern "C" int dtfa_layer_norm_fwd(const void* x, long long ldx, const float* ga
 // Workgroups (= partial rows) of the backward pass: what stays resident on 256 CUs, no more than there are rows for.
 extern "C" int dtfa_layer_norm_bwd_parts(long long rows, int cols, int dtype) {
   const long long nvec = ln_vectors(cols, dtype);
-  long long rpb = 1, most = 256;
-  if (nvec <= 128) {
-    const int tpr = nvec <= 8 ? 8 : nvec <= 16 ? 16 : nvec <= 32 ? 32 : 64;
-    rpb = 256 / tpr;
-    most = 1024;
-  } else if (nvec <= 512) {
-    rpb = nvec <= 256 ? 2 : 1;
-    most = 768;
-  } else if (nvec <= 1024) {
-    most = 512;
-  } else if (nvec > 2048) {  // column strips of the long form
+  const int tpr = nvec <= 8 ? 8 : nvec <= 16 ? 16 : nvec <= 32 ? 32 : nvec <= 256 ? 64 : nvec <= 512 ? 128 : 256;
+  const long long rpb = 256 / tpr;
+  long long most = nvec <= 64 ? 1024 : nvec <= 128 ? 768 : nvec <= 1024 ? 512 : 256;
+  if (nvec > 2048) {  // column strips of the long form
     const long long strips = (nvec + 255) / 256;
     most = strips >= 1024 ? 1 : 1024 / strips;
   }
@@ -537,9 +556,9 @@ static int ln_bwd(const LnBwd& p, long long nvec, int parts, hipStream_t st) {
   if (nvec <= 32) return ln_bwd_launch<T, 32, 1>(p, parts, st);
   if (nvec <= 64) return ln_bwd_launch<T, 64, 1>(p, parts, st);
   if (nvec <= 128) return ln_bwd_launch<T, 64, 2>(p, parts, st);
-  if (nvec <= 256) return ln_bwd_launch<T, 128, 2>(p, parts, st);
-  if (nvec <= 512) return ln_bwd_launch<T, 256, 2>(p, parts, st);
-  if (nvec <= 1024) return ln_bwd_launch<T, 512, 2>(p, parts, st);
+  if (nvec <= 256) return ln_bwd_launch<T, 64, 4>(p, parts, st);
+  if (nvec <= 512) return ln_bwd_launch<T, 128, 4>(p, parts, st);
+  if (nvec <= 1024) return ln_bwd_launch<T, 256, 4>(p, parts, st);
   if (nvec <= 2048) return ln_bwd_launch<T, 512, 4>(p, parts, st);
   if (p.dx != nullptr) {
     const long long grid = p.rows < LN_MAX_GRID ? p.rows : LN_MAX_GRID;

@@ -13,15 +13,28 @@ struct RowVec {
   typedef T V __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
 
-// The compiler would convert a vector once and keep the fp32 copies; after this it converts again.
-template <typename V>
-__device__ __forceinline__ void row_forget(V& v) {
-  typedef unsigned U __attribute__((ext_vector_type(4)));
-  static_assert(sizeof(V) == sizeof(U), "16 bytes");
-  U u = __builtin_bit_cast(U, v);
-  asm volatile("" : "+v"(u));
-  v = __builtin_bit_cast(V, u);
+// A 16-byte vector held as it is stored.  (As a vector of 16-bit elements the compiler may give every element a register
+// of its own.)
+typedef unsigned row_u32x4 __attribute__((ext_vector_type(4)));
+template <typename T>
+__device__ __forceinline__ row_u32x4 row_raw(const T* at) {
+  return __builtin_bit_cast(row_u32x4, *(const typename RowVec<T>::V*)at);
 }
+template <typename T>
+__device__ __forceinline__ float row_element(const row_u32x4& v, int j) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(v[j]);
+  } else if constexpr (__is_same(T, bf16)) {
+    return __uint_as_float(j & 1 ? v[j >> 1] & 0xffff0000u : v[j >> 1] << 16);
+  } else {
+    typedef f16 H __attribute__((ext_vector_type(2)));
+    const unsigned w = v[j >> 1];  // (by value: a vector's element has no address to cast at)
+    const H h = __builtin_bit_cast(H, w);
+    return (float)h[j & 1];
+  }
+}
+// The compiler would convert a vector once and keep the fp32 copies; after this it converts again.
+__device__ __forceinline__ void row_forget(row_u32x4& v) { asm volatile("" : "+v"(v)); }
 
 // VEC (a multiple of the 16-byte vector) consecutive elements from column `col` of a row of C as fp32; zeros behind
 // the end
