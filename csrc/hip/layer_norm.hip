@@ -11,7 +11,8 @@
 // registers over all the rows it walks: one fp32 partial row per workgroup, summed afterwards by a second kernel in a
 // fixed order, no atomics.
 //
-// A row belongs to TPR threads (a power of two, several rows to a wave below 64, a whole workgroup above), thread t
+// A row belongs to TPR threads (a power of two, chosen so that three vectors a thread are taken where two or four would
+// leave many threads without, several rows to a wave below 64, a whole workgroup above), thread t
 // holding the NV vectors t, t + TPR, ... of 16 bytes.  Rows may start at any element (odd widths, channel slices):
 // gfx950 loads and stores 16 bytes at element alignment.  The elements behind the last whole vector, fewer than eight, are
 // one more scalar in each of the first threads (with an element-wise branch per vector instead, the compiler keeps every
@@ -72,6 +73,14 @@ __device__ __forceinline__ void ln_row_sum(float (&s)[N], float* red) {
   }
 }
 
+// Whether forward workgroups walk over rows with gamma and beta in registers.  512 columns bf16: 115 -> 106 us of 2^27
+// elements, 64 columns 119 -> 113; but 512 columns fp32 95 -> 104 us of 2^26 and 1024 columns bf16 (two vectors) 97 -> 104,
+// where there are as many parameter bytes as data bytes at most and the registers cost resident waves.
+template <typename T>
+constexpr bool ln_walks(int nv) {
+  return nv == 1 && sizeof(T) == 2;
+}
+
 struct LnFwd {
   const void* x;
   long long ldx;
@@ -96,22 +105,49 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(L
   const int rest = p.cols % VEC, whole = p.cols - rest;  // the elements behind the last whole vector: one a thread
   const float n_c = (float)p.cols;  // (divided by, not multiplied with its inverse: the mean of equal values is that value)
   // (every thread of a wave takes part in the shuffles, and every thread of a workgroup in the barriers: the loop runs
-  // by the workgroup's first row, rows past the end are computed from row 0 and not stored)
-  for (long long base = (long long)blockIdx.x * RPB; base < p.rows; base += (long long)gridDim.x * RPB) {
-    const long long row = base + ln_row_of_thread<TPR, BLOCK>();
-    const bool live = row < p.rows;
-    const T* xr = (const T*)p.x + (live ? row : 0) * p.ldx;
-    // held as stored and converted at each use: half the registers of fp32 copies, and it is resident waves that keep
-    // enough loads in flight
-    row_u32x4 v[NV];
-    float e = 0.f, s[1];
+  // by the workgroup's first row, a row past the end is zeros and not stored)
+  // held as stored and converted at each use: half the registers of fp32 copies, and it is resident waves that keep
+  // enough loads in flight.  Workgroups on short rows walk many of them, the next one on its way, with gamma and beta
+  // in registers: read again for every row, these are four times the bytes of a bf16 row from the L1.
+  constexpr bool AHEAD = ln_walks<T>(NV);
+  float gam[AHEAD ? NV : 1][VEC], bet[AHEAD ? NV : 1][VEC];
+  if (AHEAD)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * TPR + t) * VEC;
-      v[i] = row_u32x4{0, 0, 0, 0};
-      if (col < whole) v[i] = row_raw<T>(xr + col);
+      if (col < whole) {
+        ln_param<VEC>(p.gamma, col, 1.f, gam[i]);
+        ln_param<VEC>(p.beta, col, 0.f, bet[i]);
+      }
     }
-    if (t < rest) e = (float)xr[whole + t];
+  struct Row {
+    row_u32x4 v[NV];
+    float e;
+  };
+  auto fetch = [&](long long base, Row& f) {
+    const long long row = base + ln_row_of_thread<TPR, BLOCK>();
+    const bool live = row < p.rows;
+    const T* xr = (const T*)p.x + row * p.ldx;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = (i * TPR + t) * VEC;
+      f.v[i] = row_u32x4{0, 0, 0, 0};
+      if (live && col < whole) f.v[i] = row_raw<T>(xr + col);
+    }
+    f.e = live && t < rest ? (float)xr[whole + t] : 0.f;
+  };
+  const long long stride = (long long)gridDim.x * RPB;
+  long long base = (long long)blockIdx.x * RPB;
+  Row r, next;
+  if (AHEAD && base < p.rows) fetch(base, r);
+  for (; base < p.rows; base += stride) {
+    const long long row = base + ln_row_of_thread<TPR, BLOCK>();
+    const bool live = row < p.rows;
+    if (!AHEAD) fetch(base, r);
+    if (AHEAD && base + stride < p.rows) fetch(base + stride, next);
+    row_u32x4(&v)[NV] = r.v;
+    const float e = r.e;
+    float s[1];
     s[0] = e;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -139,11 +175,15 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(L
         row_forget(v[i]);
         if (col < whole) {
           float g[VEC], b[VEC];
-          ln_param<VEC>(p.gamma, col, 1.f, g);
-          ln_param<VEC>(p.beta, col, 0.f, b);
+          if (!AHEAD) {
+            ln_param<VEC>(p.gamma, col, 1.f, g);
+            ln_param<VEC>(p.beta, col, 0.f, b);
+          }
           V o;
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) o[j] = (T)((row_element<T>(v[i], j) - mean) * rstd * g[j] + b[j]);
+          for (int j = 0; j < VEC; ++j)
+            o[j] = (T)((row_element<T>(v[i], j) - mean) * rstd * (AHEAD ? gam[AHEAD ? i : 0][j] : g[j])
+                       + (AHEAD ? bet[AHEAD ? i : 0][j] : b[j]));
           *(V*)(yr + col) = o;
         }
       }
@@ -156,6 +196,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(L
         p.rstd[row] = rstd;
       }
     }
+    if (AHEAD) r = next;
   }
 }
 
@@ -488,7 +529,8 @@ template <typename T, int TPR, int NV>
 static int ln_fwd_launch(const LnFwd& p, hipStream_t st) {
   constexpr int BLOCK = TPR < 256 ? 256 : TPR, RPB = BLOCK / TPR;
   long long grid = (p.rows + RPB - 1) / RPB;
-  if (grid > LN_MAX_GRID) grid = LN_MAX_GRID;
+  const long long most = ln_walks<T>(NV) ? 2048 : LN_MAX_GRID;  // (where rows are fetched ahead: what is resident)
+  if (grid > most) grid = most;
   hipLaunchKernelGGL((layer_norm_fwd_kernel<T, TPR, NV>), dim3((unsigned)grid), dim3(BLOCK), 0, st, p);
   return (int)hipGetLastError();
 }
@@ -497,9 +539,13 @@ template <typename T>
 static int ln_fwd(const LnFwd& p, long long nvec, hipStream_t st) {
   if (nvec <= 8) return ln_fwd_launch<T, 8, 1>(p, st);
   if (nvec <= 16) return ln_fwd_launch<T, 16, 1>(p, st);
+  if (nvec <= 24) return ln_fwd_launch<T, 8, 3>(p, st);
   if (nvec <= 32) return ln_fwd_launch<T, 32, 1>(p, st);
+  if (nvec <= 48) return ln_fwd_launch<T, 16, 3>(p, st);
   if (nvec <= 64) return ln_fwd_launch<T, 64, 1>(p, st);
+  if (nvec <= 96) return ln_fwd_launch<T, 32, 3>(p, st);
   if (nvec <= 128) return ln_fwd_launch<T, 64, 2>(p, st);
+  if (nvec <= 192) return ln_fwd_launch<T, 64, 3>(p, st);
   if (nvec <= 256) return ln_fwd_launch<T, 64, 4>(p, st);
   if (nvec <= 512) return ln_fwd_launch<T, 256, 2>(p, st);
   if (nvec <= 1024) return ln_fwd_launch<T, 256, 4>(p, st);
@@ -528,9 +574,11 @@ extern "C" int dtfa_layer_norm_fwd(const void* x, long long ldx, const float* ga
 // Workgroups (= partial rows) of the backward pass: what stays resident on 256 CUs, no more than there are rows for.
 extern "C" int dtfa_layer_norm_bwd_parts(long long rows, int cols, int dtype) {
   const long long nvec = ln_vectors(cols, dtype);
-  const int tpr = nvec <= 8 ? 8 : nvec <= 16 ? 16 : nvec <= 32 ? 32 : nvec <= 256 ? 64 : nvec <= 512 ? 128 : 256;
+  const int tpr = nvec <= 8 ? 8 : nvec <= 16 ? 16 : nvec <= 24 ? 8 : nvec <= 32 ? 32 : nvec <= 48 ? 16 : nvec <= 64 ? 64
+                  : nvec <= 96 ? 32 : nvec <= 256 ? 64 : nvec <= 512 ? 128 : 256;
+  const int nv = (int)((nvec + tpr - 1) / tpr);
   const long long rpb = 256 / tpr;
-  long long most = nvec <= 64 ? 1024 : nvec <= 128 ? 768 : nvec <= 1024 ? 512 : 256;
+  long long most = nv <= 1 ? 1024 : nv <= 2 ? 768 : nvec <= 1024 ? 512 : 256;
   if (nvec > 2048) {  // column strips of the long form
     const long long strips = (nvec + 255) / 256;
     most = strips >= 1024 ? 1 : 1024 / strips;
@@ -553,9 +601,13 @@ template <typename T>
 static int ln_bwd(const LnBwd& p, long long nvec, int parts, hipStream_t st) {
   if (nvec <= 8) return ln_bwd_launch<T, 8, 1>(p, parts, st);
   if (nvec <= 16) return ln_bwd_launch<T, 16, 1>(p, parts, st);
+  if (nvec <= 24) return ln_bwd_launch<T, 8, 3>(p, parts, st);
   if (nvec <= 32) return ln_bwd_launch<T, 32, 1>(p, parts, st);
+  if (nvec <= 48) return ln_bwd_launch<T, 16, 3>(p, parts, st);
   if (nvec <= 64) return ln_bwd_launch<T, 64, 1>(p, parts, st);
+  if (nvec <= 96) return ln_bwd_launch<T, 32, 3>(p, parts, st);
   if (nvec <= 128) return ln_bwd_launch<T, 64, 2>(p, parts, st);
+  if (nvec <= 192) return ln_bwd_launch<T, 64, 3>(p, parts, st);
   if (nvec <= 256) return ln_bwd_launch<T, 64, 4>(p, parts, st);
   if (nvec <= 512) return ln_bwd_launch<T, 128, 4>(p, parts, st);
   if (nvec <= 1024) return ln_bwd_launch<T, 256, 4>(p, parts, st);
