@@ -68,6 +68,8 @@ struct NsArgs {
   const NsJob* poly;        // tiles of B, tj <= ti
   const NsJob* poly_joins;
   const NsJob* full;        // tiles of X
+  const NsJob* small;       // slices of matrices whose shorter side is at most 64 (then there are no other jobs)
+  int nsmall, small_slices;
   int nchunks, npacks, ngram, ngram_joins, npoly, npoly_joins, nfull;
   int steps;
   int dtype, pad;      // of `in` (and `out`): IO_*
@@ -162,6 +164,22 @@ __device__ __forceinline__ void ns_put(f16* at, const float (&v)[8]) {
   *(f16x8*)(at + 32) = l;
 }
 
+// What G is multiplied with for X_0 as it is held, and e_0, from the partial sums; `red` is LDS for four values.
+__device__ __forceinline__ double ns_first_scale(const NsArgs& p, const NsMat& m, double* red, int& lift) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < m.parts; i += 256) s += p.part[m.part + i];
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3]));
+  const double size = norm / (norm + (double)p.eps);
+  lift = 0;
+  if (size > 0.0 && size < 1.0) (void)frexp(size, &lift);   // size * 2^-lift in [0.5, 1)
+  lift = lift < 0 ? -lift : 0;
+  return ldexp((double)m.scale / (norm + (double)p.eps), lift);
+}
+
 // X_0 times S as two fp16 planes, zeros in the padding.  A workgroup writes 64 x 64 values; its reads are on their way
 // while the norm is put together.
 template <typename T, bool MOMENTUM>
@@ -185,19 +203,9 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(NsArgs p) {
       if (MOMENTUM) row_load<float, 8>(buf + (size_t)row * m.cols, col, m.cols, b[h]);
     }
   }
-  double s = 0.0;
-  for (int i = threadIdx.x; i < m.parts; i += 256) s += p.part[m.part + i];
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-  __syncthreads();
-  const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3]));
-  int lift = 0;
-  const double size = norm / (norm + (double)p.eps);
-  if (size > 0.0 && size < 1.0) (void)frexp(size, &lift);   // size * 2^-lift in [0.5, 1)
-  lift = lift < 0 ? -lift : 0;
+  int lift;
+  const double scale = ns_first_scale(p, m, red, lift);
   if (job.y == 0 && job.z == 0 && threadIdx.x == 0) p.part[p.nparts + job.x] = (double)lift;
-  const double scale = ldexp((double)m.scale / (norm + (double)p.eps), lift);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -501,6 +509,25 @@ __device__ __forceinline__ void ns_join_slabs(const NsArgs& p, const NsMat& m, c
 
 enum { NS_NEXT = 0, NS_OUT = 1, NS_APPLY = 2 };
 
+// Eight consecutive values of the result, into the output or the parameters.
+template <int WHAT, typename O>
+__device__ __forceinline__ void ns_result(const NsArgs& p, const NsMat& m, int row, int col, const float* o, float keep, float rate) {
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = o[j];
+  const size_t flat = m.at + (size_t)row * m.cols;
+  if (WHAT == NS_OUT) {
+    row_store<O, 8>((O*)p.out + flat, col, m.cols, v);
+  } else {
+    float w[8];
+    row_load<float, 8>(p.w + flat, col, m.cols, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = w[j] * keep - rate * v[j];
+    row_store<float, 8>(p.w + flat, col, m.cols, w);
+    if (p.w16 != nullptr) row_store<bf16, 8>(p.w16 + flat, col, m.cols, w);
+  }
+}
+
 // Tile of a X + B X (or a X + X B): the next iterate, the result, or the parameter update with it.
 template <int T, int WHAT, typename O>
 __device__ __forceinline__ void ns_advance(const NsArgs& p, const NsMat& m, const NsJob& job, int k, int lift, int lift_next,
@@ -538,17 +565,7 @@ __device__ __forceinline__ void ns_advance(const NsArgs& p, const NsMat& m, cons
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= unscale;
-    const size_t flat = m.at + (size_t)row * m.cols;
-    if (WHAT == NS_OUT) {
-      row_store<O, 8>((O*)p.out + flat, col, m.cols, v);
-    } else {
-      float w[8];
-      row_load<float, 8>(p.w + flat, col, m.cols, w);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = w[j] * keep - rate * v[j];
-      row_store<float, 8>(p.w + flat, col, m.cols, w);
-      if (p.w16 != nullptr) row_store<bf16, 8>(p.w16 + flat, col, m.cols, w);
-    }
+    ns_result<WHAT, O>(p, m, row, col, v, keep, rate);
   }
 }
 
@@ -592,6 +609,252 @@ __global__ __launch_bounds__(256, 2) void ns_advance_kernel(NsArgs p, int k) {
     ns_advance<64, WHAT, O>(p, m, job, k, lift, lift_next, smem);
 }
 
+// ---------------------------------------------------------------- short sides of at most 64
+// One launch an iteration.  A workgroup owns a slice of X, `edge` blocks of 64 x 64 along its long side, from block
+// `tj` on; A, 64 x 64, is the sum of all slices' partial products, which every workgroup of the matrix adds up for
+// itself (in slice order, so that all hold the same A) and turns into B; then it advances its blocks and leaves the partial
+// product of the new ones.  64 x 576 is a chain of small launches whatever is done: three an iteration took 15 us,
+// bound by their own latency; this one takes NS_SMALL_US.
+//
+// Tiles in LDS: 64 rows of 256 bytes, two blocks of 32 columns, hi and lo.  One swizzle serves both ways of reading:
+// 16 rows at one chunk (all four bits of the row differ) and 64 bytes in four consecutive rows (its low bits on top).
+#define NS_TILE 16384
+__device__ __forceinline__ int ns_mix(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }
+// byte offset of the 16-byte chunk that holds (row, col)
+__device__ __forceinline__ int ns_chunk(int row, int col, int lo) {
+  return row * 256 + ((((col >> 5) * 8 + lo * 4 + ((col & 31) >> 3)) ^ ns_mix(row)) << 4);
+}
+
+// 64 x 64 product of two tiles over 64 k, added to `acc`; the wave's quarter, transposed as in ns_product
+template <bool PK, bool QK>
+__device__ __forceinline__ void ns_small_product(const char* P, const char* Q, f32x16& acc) {
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const int tr_k = 8 * (lane >> 5) + ((lane & 15) >> 2), tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  auto frag = [&](const char* tile, bool km, int row0, int kk, int lo) -> f16x8 {
+    if (km) {
+      union { s16x4 h[2]; f16x8 v; } r;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int krow = kk * 16 + tr_k + 4 * q;
+        const char* at = tile + ns_chunk(krow, row0 + tr_col, lo) + (tr_col & 7) * 2;
+        r.h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)at);
+      }
+      return r.v;
+    }
+    return *(const f16x8*)(tile + ns_chunk(row0 + (lane & 31), kk * 16 + (lane >> 5) * 8, lo));
+  };
+  const int i0 = (wid >> 1) * 32, j0 = (wid & 1) * 32;
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk) {
+    const f16x8 ph = frag(P, PK, i0, kk, 0), qh = frag(Q, QK, j0, kk, 0);
+    const f16x8 pl = frag(P, PK, i0, kk, 1), ql = frag(Q, QK, j0, kk, 1);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, ph, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql, ph, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, pl, acc, 0, 0, 0);
+  }
+}
+
+// four consecutive values of a tile, col a multiple of 4
+__device__ __forceinline__ void ns_small_get(const char* tile, int row, int col, float (&v)[4]) {
+  const int in = (col & 7) * 2;
+  const f16x4 h = *(const f16x4*)(tile + ns_chunk(row, col, 0) + in), l = *(const f16x4*)(tile + ns_chunk(row, col, 1) + in);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = (float)h[j] + (float)l[j];
+}
+__device__ __forceinline__ void ns_small_put(char* tile, int row, int col, const float (&v)[4]) {
+  f16x4 h, l;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    f16 a, b;
+    ns_split(v[j], a, b);
+    h[j] = a;
+    l[j] = b;
+  }
+  const int in = (col & 7) * 2;
+  *(f16x4*)(tile + ns_chunk(row, col, 0) + in) = h;
+  *(f16x4*)(tile + ns_chunk(row, col, 1) + in) = l;
+}
+__device__ __forceinline__ f32x16 ns_zero() {
+  f32x16 z;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) z[e] = 0.f;
+  return z;
+}
+
+// a block of X: 64 rows of 256 bytes, `ld` elements apart per plane
+__device__ __forceinline__ void ns_small_fetch(const f16* x, int ld, row_u32x4 (&v)[4]) {
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const int row = n * 16 + (threadIdx.x >> 4), chunk = threadIdx.x & 15;
+    v[n] = *(const row_u32x4*)(x + (size_t)row * 2 * ld + chunk * 8);
+  }
+}
+__device__ __forceinline__ void ns_small_to_tile(const row_u32x4 (&v)[4], char* tile) {
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const int row = n * 16 + (threadIdx.x >> 4), chunk = threadIdx.x & 15;
+    *(row_u32x4*)(tile + row * 256 + ((chunk ^ ns_mix(row)) << 4)) = v[n];
+  }
+}
+__device__ __forceinline__ void ns_small_from_tile(const char* tile, f16* x, int ld) {
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const int row = n * 16 + (threadIdx.x >> 4), chunk = threadIdx.x & 15;
+    *(row_u32x4*)(x + (size_t)row * 2 * ld + chunk * 8) = *(const row_u32x4*)(tile + row * 256 + ((chunk ^ ns_mix(row)) << 4));
+  }
+}
+// partial product of this slice: [i][j], four consecutive j a store
+__device__ __forceinline__ void ns_small_slab(const f32x16& acc, float* slab) {
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const int i = (wid >> 1) * 32 + (lane & 31), j = (wid & 1) * 32 + 4 * (lane >> 5);
+#pragma unroll
+  for (int e = 0; e < 16; e += 4)
+    *(f32x4*)(slab + i * 64 + j + 2 * e) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+}
+__device__ __forceinline__ f16* ns_small_block(const NsArgs& p, const NsMat& m, int k, int block) {
+  f16* x = p.ws + m.x + (k & 1 ? (size_t)2 * m.rp * m.cp : 0);
+  return x + (m.tall ? (size_t)block * 64 * 2 * m.cp : (size_t)block * 128);
+}
+
+// X_0 of a slice and its partial product
+template <typename T, bool MOMENTUM>
+__global__ __launch_bounds__(256) void ns_small_first_kernel(NsArgs p) {
+  __shared__ __attribute__((aligned(16))) char tile[NS_TILE];
+  __shared__ double red[4];
+  const NsJob job = p.small[blockIdx.x];
+  const NsMat m = p.mats[job.mat];
+  const T* in = (const T*)p.in + m.at;
+  const float* buf = MOMENTUM ? p.buf + m.at : nullptr;
+  const float gs = MOMENTUM ? p.hyper[1] : 1.f;
+  int lift;
+  const double scale = ns_first_scale(p, m, red, lift);
+  if (job.ti == 0 && threadIdx.x == 0) p.part[p.nparts + job.mat] = (double)lift;
+  f32x16 acc = ns_zero();
+  for (int block = job.tj; block < job.tj + job.edge; ++block) {
+    const int row0 = m.tall ? block * 64 : 0, col0 = m.tall ? 0 : block * 64;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = h * 32 + (threadIdx.x >> 3), c = (threadIdx.x & 7) * 8, row = row0 + r, col = col0 + c;
+      float g[8], b[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = b[j] = 0.f;
+      if (row < m.rows && col < m.cols) {
+        row_load<T, 8>(in + (size_t)row * m.cols, col, m.cols, g);
+        if (MOMENTUM) row_load<float, 8>(buf + (size_t)row * m.cols, col, m.cols, b);
+      }
+      f16x8 vh, vl;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (MOMENTUM) g[j] = ns_direction(g[j] * gs, b[j], p.mu, p.nesterov);
+        f16 hi, lo;
+        ns_split((float)((double)g[j] * scale), hi, lo);
+        vh[j] = hi;
+        vl[j] = lo;
+      }
+      *(f16x8*)(tile + ns_chunk(r, c, 0)) = vh;
+      *(f16x8*)(tile + ns_chunk(r, c, 1)) = vl;
+    }
+    __syncthreads();
+    if (m.tall)
+      ns_small_product<true, true>(tile, tile, acc);
+    else
+      ns_small_product<false, false>(tile, tile, acc);
+    ns_small_from_tile(tile, ns_small_block(p, m, 0, block), m.cp);
+    __syncthreads();
+  }
+  ns_small_slab(acc, p.slabs + (size_t)(job.slab + job.ti) * 4096);
+}
+
+// Iteration k of a slice; the partial products of iteration k are in half k % 2 of the slabs.
+template <int WHAT, typename O>
+__global__ __launch_bounds__(256) void ns_small_kernel(NsArgs p, int k) {
+  __shared__ __attribute__((aligned(16))) char lds[2 * NS_TILE + 64 * NS_PITCH(64) * 4];
+  char* tb = lds;                 // B
+  char* tx = lds + NS_TILE;       // A, then X
+  char* tn = lds + 2 * NS_TILE;   // the next X; its fp32 tile where it is the result
+  const NsJob job = p.small[blockIdx.x];
+  const NsMat m = p.mats[job.mat];
+  const int lift = ns_lift(p, job.mat, k), lift_next = ns_lift(p, job.mat, k + 1);
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const int i = (wid >> 1) * 32 + (lane & 31), j = (wid & 1) * 32 + 4 * (lane >> 5);
+  row_u32x4 x[4];
+  ns_small_fetch(ns_small_block(p, m, k, job.tj), m.cp, x);
+  {  // A
+    const float* slab = p.slabs + (size_t)((k & 1) * p.small_slices + job.slab) * 4096 + threadIdx.x * 4;
+    f32x4 v[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) v[n] = *(const f32x4*)(slab + n * 1024);
+#pragma unroll 2
+    for (int q = 1; q < job.k0; ++q)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) v[n] += *(const f32x4*)(slab + (size_t)q * 4096 + n * 1024);
+    const float f = NS_GRAM_SCALE / (m.scale * m.scale);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const float a[4] = {v[n][0] * f, v[n][1] * f, v[n][2] * f, v[n][3] * f};
+      ns_small_put(tx, n * 16 + (threadIdx.x >> 4), (threadIdx.x & 15) * 4, a);
+    }
+  }
+  __syncthreads();
+  {  // B
+    f32x16 acc = ns_zero();
+    ns_small_product<false, false>(tx, tx, acc);
+    const float f = ldexpf(NS_C / NS_GRAM_SCALE, -2 * lift);
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      float v[4];
+      ns_small_get(tx, i, j + 2 * e, v);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = NS_B * v[q] + f * acc[e + q];
+      ns_small_put(tb, i, j + 2 * e, v);
+    }
+  }
+  __syncthreads();
+  const float fx = ldexpf(NS_A, lift_next - lift), ft = ldexpf(1.f / NS_GRAM_SCALE, lift_next - 3 * lift);
+  const float unscale = ldexpf(1.f / m.scale, -lift_next);
+  const float lr = WHAT == NS_APPLY ? p.hyper[0] : 0.f;
+  const float keep = 1.f - lr * p.wd, rate = lr * m.lr_scale;
+  f32x16 gram = ns_zero();
+  for (int block = job.tj; block < job.tj + job.edge; ++block) {
+    ns_small_to_tile(x, tx);
+    if (block + 1 < job.tj + job.edge) ns_small_fetch(ns_small_block(p, m, k, block + 1), m.cp, x);
+    __syncthreads();
+    f32x16 acc = ns_zero();
+    if (m.tall)
+      ns_small_product<false, false>(tx, tb, acc);
+    else
+      ns_small_product<false, true>(tb, tx, acc);
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      float v[4];
+      ns_small_get(tx, i, j + 2 * e, v);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = fx * v[q] + ft * acc[e + q];
+      if (WHAT == NS_NEXT)
+        ns_small_put(tn, i, j + 2 * e, v);
+      else
+        *(f32x4*)((float*)tn + i * NS_PITCH(64) + j + 2 * e) = f32x4{v[0] * unscale, v[1] * unscale, v[2] * unscale, v[3] * unscale};
+    }
+    __syncthreads();
+    if (WHAT == NS_NEXT) {
+      if (m.tall)
+        ns_small_product<true, true>(tn, tn, gram);
+      else
+        ns_small_product<false, false>(tn, tn, gram);
+      ns_small_from_tile(tn, ns_small_block(p, m, k + 1, block), m.cp);
+    } else {
+      const int row0 = m.tall ? block * 64 : 0, col0 = m.tall ? 0 : block * 64;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = h * 32 + (threadIdx.x >> 3), c = (threadIdx.x & 7) * 8;
+        if (row0 + r < m.rows && col0 + c < m.cols) ns_result<WHAT, O>(p, m, row0 + r, col0 + c, (float*)tn + r * NS_PITCH(64) + c, keep, rate);
+      }
+    }
+    __syncthreads();
+  }
+  if (WHAT == NS_NEXT) ns_small_slab(gram, p.slabs + (size_t)((k + 1 & 1) * p.small_slices + job.slab + job.ti) * 4096);
+}
+
 // ---------------------------------------------------------------- host
 template <void (*KERNEL)(NsArgs, int)>
 static int ns_tiles(int blocks, const NsArgs& a, int k, hipStream_t st) {
@@ -615,15 +878,21 @@ static int ns_join(int tiles, const NsArgs& a, int k, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
-template <typename T>
+template <typename T, bool MOMENTUM>
 static int ns_first(const NsArgs& a, hipStream_t st) {
-  if (a.buf != nullptr) {
-    hipLaunchKernelGGL((ns_norm_kernel<T, true>), dim3(a.nchunks), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((ns_pack_kernel<T, true>), dim3(a.npacks), dim3(256), 0, st, a);
-  } else {
-    hipLaunchKernelGGL((ns_norm_kernel<T, false>), dim3(a.nchunks), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((ns_pack_kernel<T, false>), dim3(a.npacks), dim3(256), 0, st, a);
-  }
+  hipLaunchKernelGGL((ns_norm_kernel<T, MOMENTUM>), dim3(a.nchunks), dim3(256), 0, st, a);
+  if (a.nsmall > 0)
+    hipLaunchKernelGGL((ns_small_first_kernel<T, MOMENTUM>), dim3(a.nsmall), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((ns_pack_kernel<T, MOMENTUM>), dim3(a.npacks), dim3(256), 0, st, a);
+  return (int)hipGetLastError();
+}
+
+// the advancing stage of iteration k
+template <int WHAT, typename O>
+static int ns_step(const NsArgs& a, int k, hipStream_t st) {
+  if (a.nsmall == 0) return ns_tiles<ns_advance_kernel<WHAT, O>>(a.nfull, a, k, st);
+  hipLaunchKernelGGL((ns_small_kernel<WHAT, O>), dim3(a.nsmall), dim3(256), 0, st, a, k);
   return (int)hipGetLastError();
 }
 
@@ -631,27 +900,35 @@ static int ns_first(const NsArgs& a, hipStream_t st) {
 // or the parameters.
 extern "C" int dtfa_newton_schulz(const NsArgs* args, hipStream_t st) {
   const NsArgs a = *args;
-  if (a.nchunks <= 0 || a.npacks <= 0 || a.ngram <= 0 || a.npoly <= 0 || a.nfull <= 0 || a.steps < 1) return -1;
-  if ((a.out == nullptr) == (a.w == nullptr) || (a.w != nullptr && (a.buf == nullptr || a.hyper == nullptr))) return -2;
-  if (a.out == nullptr && a.dtype == IO_F16) return -3;
-  int rc = a.dtype == IO_BF16 ? ns_first<bf16>(a, st) : a.dtype == IO_F16 ? ns_first<f16>(a, st)
-           : a.dtype == IO_F32 ? ns_first<float>(a, st) : -3;
+  if (a.nchunks <= 0 || a.steps < 1) return -1;
+  if (a.nsmall <= 0 && (a.npacks <= 0 || a.ngram <= 0 || a.npoly <= 0 || a.nfull <= 0)) return -1;
+  if ((a.out == nullptr) == (a.w == nullptr) || (a.w != nullptr) != (a.buf != nullptr) || (a.w != nullptr && a.hyper == nullptr))
+    return -2;
+  if (a.dtype != IO_BF16 && a.dtype != IO_F32 && (a.dtype != IO_F16 || a.buf != nullptr)) return -3;
+  int rc;
+  if (a.buf != nullptr)
+    rc = a.dtype == IO_BF16 ? ns_first<bf16, true>(a, st) : ns_first<float, true>(a, st);
+  else
+    rc = a.dtype == IO_BF16 ? ns_first<bf16, false>(a, st) : a.dtype == IO_F16 ? ns_first<f16, false>(a, st)
+         : ns_first<float, false>(a, st);
   for (int k = 0; k < a.steps && rc == 0; ++k) {
-    rc = ns_tiles<ns_symmetric_kernel<false>>(a.ngram, a, k, st);
-    if (rc == 0 && a.ngram_joins > 0) rc = ns_join<false>(a.ngram_joins, a, k, st);
-    if (rc == 0) rc = ns_tiles<ns_symmetric_kernel<true>>(a.npoly, a, k, st);
-    if (rc == 0 && a.npoly_joins > 0) rc = ns_join<true>(a.npoly_joins, a, k, st);
-    if (rc != 0) break;
+    if (a.nsmall == 0) {
+      rc = ns_tiles<ns_symmetric_kernel<false>>(a.ngram, a, k, st);
+      if (rc == 0 && a.ngram_joins > 0) rc = ns_join<false>(a.ngram_joins, a, k, st);
+      if (rc == 0) rc = ns_tiles<ns_symmetric_kernel<true>>(a.npoly, a, k, st);
+      if (rc == 0 && a.npoly_joins > 0) rc = ns_join<true>(a.npoly_joins, a, k, st);
+      if (rc != 0) break;
+    }
     if (k + 1 < a.steps)
-      rc = ns_tiles<ns_advance_kernel<NS_NEXT, float>>(a.nfull, a, k, st);
+      rc = ns_step<NS_NEXT, float>(a, k, st);
     else if (a.out == nullptr)
-      rc = ns_tiles<ns_advance_kernel<NS_APPLY, float>>(a.nfull, a, k, st);
+      rc = ns_step<NS_APPLY, float>(a, k, st);
     else if (a.dtype == IO_BF16)
-      rc = ns_tiles<ns_advance_kernel<NS_OUT, bf16>>(a.nfull, a, k, st);
+      rc = ns_step<NS_OUT, bf16>(a, k, st);
     else if (a.dtype == IO_F16)
-      rc = ns_tiles<ns_advance_kernel<NS_OUT, f16>>(a.nfull, a, k, st);
+      rc = ns_step<NS_OUT, f16>(a, k, st);
     else
-      rc = ns_tiles<ns_advance_kernel<NS_OUT, float>>(a.nfull, a, k, st);
+      rc = ns_step<NS_OUT, float>(a, k, st);
   }
   return rc;
 }

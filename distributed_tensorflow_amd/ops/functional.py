@@ -1045,7 +1045,11 @@ class _LayerNormFn(Function):
         want_dx, want_dg, want_db = ctx.needs_input_grad[:3]
         dx, dg, db = K.layer_norm_bwd(dy, x, gamma, stats, want_dx, want_dg, want_db)
         pg, pb = ctx.params
-        return dx, _deliver_small(pg, dg), _deliver_small(pb, db), None, None
+        if hasattr(pg, "main_grad"):
+            dg = _deliver_small(pg, dg)
+        if hasattr(pb, "main_grad"):
+            db = _deliver_small(pb, db)
+        return dx, dg, db, None, None
 
 
 def layer_norm(x, gamma=None, beta=None, eps: float = 1e-5):

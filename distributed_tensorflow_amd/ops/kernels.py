@@ -556,6 +556,11 @@ def _ln_rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     return t.contiguous(), cols
 
 
+def _ln_like(x: torch.Tensor) -> torch.Tensor:
+    # (a contiguous result whatever x's layout; empty_like costs half of empty with everything spelt out)
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def _ln_check(x: torch.Tensor, gamma, beta) -> None:
     if not x.is_cuda:
         raise ValueError("layer_norm: x must be a GPU tensor")
@@ -580,7 +585,7 @@ def layer_norm_fwd(x: torch.Tensor, gamma: Optional[torch.Tensor], beta: Optiona
     cols = x.shape[-1]
     rows = x.numel() // cols
     with hipk.device_of(x):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = _ln_like(x)
         stats = torch.empty((2, rows), dtype=F32, device=x.device) if want_stats else None
         if rows:
             xr, ldx = _ln_rows(x)
@@ -605,7 +610,7 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, gamma: Optional[torch.Tens
         raise ValueError("layer_norm backward: stats must be two values for each of %d rows, got shape %s"
                          % (rows, tuple(stats.shape)))
     with hipk.device_of(x):
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
+        dx = _ln_like(x) if want_dx else None
         fresh = torch.empty if rows else torch.zeros
         dgamma = fresh(cols, dtype=F32, device=x.device) if want_dgamma else None
         dbeta = fresh(cols, dtype=F32, device=x.device) if want_dbeta else None
@@ -614,7 +619,7 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, gamma: Optional[torch.Tens
             (xr, ldx), (gr, ldg) = _ln_rows(x), _ln_rows(dy)
             part = None
             if want_dgamma or want_dbeta:
-                part = torch.empty((L.dtfa_layer_norm_bwd_parts(rows, cols, dt), 2, cols), dtype=F32, device=x.device)
+                part = torch.empty(L.dtfa_layer_norm_bwd_parts(rows, cols, dt) * 2 * cols, dtype=F32, device=x.device)
             hipk.check(L.dtfa_layer_norm_bwd(xr.data_ptr(), ldx, gr.data_ptr(), ldg, hipk.ptr(gamma), stats.data_ptr(),
                                              hipk.ptr(dx), hipk.ptr(part), hipk.ptr(dgamma), hipk.ptr(dbeta), rows, cols, dt, hipk.stream()), "layer_norm_bwd")
     return dx, dgamma, dbeta

@@ -33,6 +33,12 @@ CUS = 256
 SLOTS = 2 * CUS           # workgroups at a time
 MIN_STEPS = 8             # shortest piece of a cut reduction
 
+# Shorter sides of at most 64 take one launch an iteration, in which every workgroup adds up the partial products of all
+# slices of its matrix (0.35 us each) and advances the 64 x 64 blocks of its own (1.2 us each): the time is least
+# at sqrt(1.2 / 0.35 * blocks) slices, and beyond 128 blocks the separate stages are faster.
+SMALL_BLOCKS_PER_SLICE2 = 1.2 / 0.35
+SMALL_MAX_LONG = 8192
+
 _MAT = np.dtype([("at", "<i8"), ("x", "<i8"), ("a", "<i8"), ("part", "<i8"), ("rows", "<i4"), ("cols", "<i4"),
                  ("rp", "<i4"), ("cp", "<i4"), ("mp", "<i4"), ("parts", "<i4"), ("chunk", "<i4"), ("tall", "<i4"),
                  ("scale", "<f4"), ("lr_scale", "<f4")])   # NsMat
@@ -40,7 +46,8 @@ _MAT = np.dtype([("at", "<i8"), ("x", "<i8"), ("a", "<i8"), ("part", "<i8"), ("r
 
 class NsArgs(C.Structure):
     _fields_ = [("mats", C.c_void_p), ("chunks", C.c_void_p), ("packs", C.c_void_p), ("gram", C.c_void_p), ("joins", C.c_void_p),
-                ("poly", C.c_void_p), ("poly_joins", C.c_void_p), ("full", C.c_void_p), ("nchunks", C.c_int),
+                ("poly", C.c_void_p), ("poly_joins", C.c_void_p), ("full", C.c_void_p), ("small", C.c_void_p), ("nsmall", C.c_int),
+                ("small_slices", C.c_int), ("nchunks", C.c_int),
                 ("npacks", C.c_int), ("ngram", C.c_int), ("ngram_joins", C.c_int), ("npoly", C.c_int),
                 ("npoly_joins", C.c_int), ("nfull", C.c_int), ("steps", C.c_int), ("dtype", C.c_int), ("pad", C.c_int), ("in_", C.c_void_p), ("out", C.c_void_p), ("buf", C.c_void_p),
                 ("w", C.c_void_p), ("w16", C.c_void_p), ("hyper", C.c_void_p), ("part", C.c_void_p), ("slabs", C.c_void_p), ("ws", C.c_void_p), ("nparts", C.c_longlong),
@@ -147,10 +154,16 @@ def _cut_tail(jobs: np.ndarray, slabs: int) -> Tuple[np.ndarray, np.ndarray, int
     return np.concatenate([jobs[:-tail], cut]), joins, slabs
 
 
+def _join(parts: Sequence[np.ndarray], width: int = 8) -> np.ndarray:
+    return np.concatenate(parts) if parts else np.zeros((0, width), dtype=np.int32)
+
+
 def _over_xcds(groups: Sequence[np.ndarray]) -> np.ndarray:
     """Workgroup n runs on XCD n % 8, each with its own L2: neighbouring tiles, which read the same rows, go to the same
     XCD.  Every run of equal jobs is dealt out in eight consecutive parts, what does not divide job by job to the XCDs
     with the least work so far; within an XCD the longest jobs start first.  Shorter queues end in empty jobs."""
+    if not groups:
+        return _join(groups)
     runs = []
     for g in groups:
         runs += np.split(g, np.flatnonzero(np.diff(_cost(g))) + 1)
@@ -184,11 +197,13 @@ class NsPlan:
         for _, rows, cols in matrices:
             check_shape(rows, cols, "orthogonalize")
         sides = [(min(rows, cols), max(rows, cols)) for _, rows, cols in matrices]
+        fused = max(short for short, _ in sides) <= 64 and max(long for _, long in sides) <= SMALL_MAX_LONG
         gram_large, gram_piece = _choose([(short, short, long) for short, long in sides], True)
         poly_large, poly_piece = _choose([(short, short, short) for short, _ in sides], True)
         full_large, _ = _choose([(short, long, short) for short, long in sides], False)
         chunks, packs, gram, gram_joins, poly, poly_joins, full = [], [], [], [], [], [], []
-        ws = part = gram_slabs = poly_slabs = 0
+        small: List[np.ndarray] = []
+        ws = part = gram_slabs = poly_slabs = small_slices = 0
         for k, (at, rows, cols) in enumerate(matrices):
             short = min(rows, cols)
             edge = 128 if short >= min(gram_large, poly_large, full_large) else 64
@@ -201,6 +216,13 @@ class NsPlan:
                        math.sqrt(max(1.0, rows / cols)))
             ws += 4 * rp * cp + 4 * mp * mp
             part += parts
+            if fused:
+                blocks = max(rp, cp) // 64
+                slices = min(blocks, max(1, round(math.sqrt(SMALL_BLOCKS_PER_SLICE2 * blocks))))
+                edges = np.arange(slices + 1) * blocks // slices
+                jobs = _jobs(k, np.arange(slices), edges[:-1], np.diff(edges), slices, 0, small_slices)
+                small.append(jobs)
+                small_slices += slices
             chunks.append(np.stack([np.full(parts, k), np.arange(parts), np.zeros(parts), np.zeros(parts)], 1).astype(np.int32))
             i, j = _tiles(rp // 64, cp // 64)
             packs.append(np.stack([np.full_like(i, k), i, j, np.zeros_like(i)], 1).astype(np.int32))
@@ -219,15 +241,19 @@ class NsPlan:
             poly_joins.append(joins)
             e = 128 if short >= full_large else 64
             full.append(_jobs(k, *_tiles(rp // e, cp // e), e, 0, mp))
+        if fused:   # one launch an iteration, no other jobs
+            packs, gram, gram_joins, poly, poly_joins, full = [], [], [], [], [], []
+            gram_slabs, poly_slabs = 2 * small_slices, 0
         slabs = max(gram_slabs, poly_slabs)   # (a stage's slabs are joined before the next stage writes its own)
-        lists = [np.concatenate(chunks), np.concatenate(packs), _over_xcds(gram), np.concatenate(gram_joins),
-                 _over_xcds(poly), np.concatenate(poly_joins), _over_xcds(full)]
-        self.counts = [len(v) for v in lists]
+        lists = [np.concatenate(chunks), _join(packs, 4), _over_xcds(gram), _join(gram_joins), _over_xcds(poly),
+                 _join(poly_joins), _over_xcds(full), _join(small)]
+        counts = [len(v) for v in lists]
+        self.counts = [counts[7], small_slices] + counts[:7]
         # 32-byte aligned: the lists are read 16 and 32 bytes at a time
         blobs = [v.tobytes() + b"\0" * (-v.nbytes % 32) for v in [mats] + lists]
         self.table = torch.from_numpy(np.frombuffer(b"".join(blobs), dtype=np.uint8).copy()).to(device)
         starts = np.cumsum([0] + [len(v) for v in blobs])
-        self.places = [self.table.data_ptr() + int(s) for s in starts[:8]]
+        self.places = [self.table.data_ptr() + int(s) for s in starts[:9]]
         self.ws_elems, self.parts, self.mats, self.slabs = ws, part, len(matrices), slabs
 
     def launch(self, *, inp: torch.Tensor, steps: int, out=None, buf=None, w=None, w16=None, hyper=None, mu=0.0,

@@ -53,7 +53,7 @@ def _matrix(rows, cols, dtype, seed, kind="noise"):
 
 
 SIZES = [(1, 1), (1, 7), (7, 1), (3, 3), (8, 1024), (32, 72), (64, 64), (65, 63), (64, 576), (63, 300), (300, 63), (129, 1000),
-         (512, 512), (515, 513), (512, 1030), (1000, 515), (640, 2049), (2049, 640)]
+         (512, 512), (515, 513), (512, 1030), (1000, 515), (640, 2049), (2049, 640), (64, 8192), (8200, 64), (40, 1500), (1500, 17), (1, 4000), (64, 8300)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
@@ -264,6 +264,33 @@ def test_step(grad_dtype, nesterov):
         assert torch.equal(region.w16[s], region.w[s].bfloat16())
     assert torch.equal(got_w[~inside], w[~inside].double()) and torch.equal(got_buf[~inside], buf[~inside].double())
     assert torch.equal(got_w16[~inside], w.bfloat16()[~inside].double())
+
+
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_step_over_short_matrices(nesterov):
+    # all sides of at most 64: one launch an iteration
+    places = [(0, 8, 1024), (8192, 64, 576), (45056, 500, 33), (61568, 7, 5), (61632, 64, 64)]
+    total = 65792
+    gen = torch.Generator().manual_seed(33)
+    w, g, buf = (torch.randn(total, generator=gen) * s for s in (1.0, 1e-3, 1e-2))
+    region = OptRegion("r", w.cuda(), g.cuda(), w.bfloat16().cuda(), True, places)
+    opt = make_optimizer("muon", [region], 0.02, nesterov=nesterov, weight_decay=0.1)
+    opt.buf["r"].copy_(buf)
+    opt.step()
+    m = 0.95 * buf.double() + g.double()
+    u = g.double() + 0.95 * m if nesterov else m
+    inside = torch.zeros(total, dtype=torch.bool)
+    for at, r, c in places:
+        s = slice(at, at + r * c)
+        inside[s] = True
+        d = u[s].view(r, c)
+        o = ref.newton_schulz(d, 5)
+        rate = 0.02 * math.sqrt(max(1, r / c))
+        want = w[s].double() * (1 - 0.02 * 0.1) - rate * o.view(-1)
+        off = (region.w[s].double().cpu() - want).norm().item()
+        assert off <= rate * _allowed(d, o) * 2 + 4 * 2.0 ** -24 * w[s].double().norm().item(), (r, c)
+        assert torch.equal(region.w16[s], region.w[s].bfloat16())
+    assert torch.equal(region.w.cpu()[~inside], w[~inside])
 
 
 def test_step_without_bf16_copy_and_with_vectors():

@@ -62,7 +62,7 @@ def test_refusals():
         F.orthogonalize(torch.nn.Parameter(x))
 
 
-@pytest.mark.parametrize("shapes", [[(1, 1)], [(64, 64), (65, 64)], [(5, 700), (700, 5), (513, 2000), (1031, 600)],
+@pytest.mark.parametrize("shapes", [[(64, 64), (65, 80)], [(5, 700), (700, 5), (513, 2000), (1031, 600)],
                                     [(2048, 512), (64, 64), (1000, 2048)], [(4096, 4096)], [(4700, 3900)],
                                     [(256, 2304)] * 6])
 def test_plan_covers_every_tile_once_and_stays_inside(shapes):
@@ -74,10 +74,12 @@ def test_plan_covers_every_tile_once_and_stays_inside(shapes):
     table, base = plan.table.numpy(), plan.table.data_ptr()
     mats = table[:len(shapes) * ns._MAT.itemsize].view(ns._MAT)
     lists = []
-    for start, count, width in zip(plan.places[1:], plan.counts, (4, 4, 8, 8, 8, 8, 8)):
+    counts = plan.counts[2:] + plan.counts[:1]
+    for start, count, width in zip(plan.places[1:], counts, (4, 4, 8, 8, 8, 8, 8, 8)):
         assert (start - base) % 32 == 0 and start - base + 4 * width * count <= table.size
         lists.append(table[start - base:start - base + 4 * width * count].view(np.int32).reshape(-1, width))
-    chunks, packs, gram, gram_joins, poly, poly_joins, full = lists
+    chunks, packs, gram, gram_joins, poly, poly_joins, full, small = lists
+    assert not len(small)
     end = part = 0
     slabs = {id(gram): [], id(poly): [], id(full): []}   # (first, length) of every tile's slabs
     for k, (m, (at, r, c)) in enumerate(zip(mats, places)):
@@ -124,6 +126,32 @@ def test_plan_covers_every_tile_once_and_stays_inside(shapes):
         places = sorted(zip(v[::2], v[1::2]))
         assert all(a + n == b for (a, n), (b, _) in zip(places, places[1:])) and (not places or places[0][0] == 0)
         assert not places or sum(places[-1]) <= plan.slabs
+
+
+@pytest.mark.parametrize("shapes", [[(1, 1)], [(64, 576)] * 3, [(5, 700), (700, 5), (64, 64), (33, 8192)]])
+def test_short_sides_are_sliced_completely(shapes):
+    places, at = [], 0
+    for r, c in shapes:
+        places.append((at, r, c))
+        at += r * c
+    plan = ns.NsPlan(places, "cpu")
+    table, base = plan.table.numpy(), plan.table.data_ptr()
+    mats = table[:len(shapes) * ns._MAT.itemsize].view(ns._MAT)
+    nsmall, slices = plan.counts[:2]
+    assert nsmall == slices and plan.counts[3:] == [0] * 6 and plan.slabs == 2 * slices
+    start = plan.places[8] - base
+    jobs = table[start:start + 32 * nsmall].view(np.int32).reshape(-1, 8)
+    slab = 0
+    for k, m in enumerate(mats):
+        mine = jobs[jobs[:, 0] == k]
+        blocks = max(m["rp"], m["cp"]) // 64
+        assert min(m["rp"], m["cp"]) == m["mp"] == 64
+        # {matrix, slice, first block, blocks, slices, -, first slab, -}: slice after slice, block after block
+        assert list(mine[:, 1]) == list(range(len(mine))) and (mine[:, 3] >= 1).all() and (mine[:, 4] == len(mine)).all()
+        assert mine[0, 2] == 0 and (mine[1:, 2] == mine[:-1, 2] + mine[:-1, 3]).all() and mine[-1, 2] + mine[-1, 3] == blocks
+        assert (mine[:, 6] == slab).all()
+        slab += len(mine)
+    assert slab == slices
 
 
 def _model():
