@@ -72,7 +72,8 @@ struct NsArgs {
   int nsmall, small_slices;
   int nchunks, npacks, ngram, ngram_joins, npoly, npoly_joins, nfull;
   int steps;
-  int dtype, pad;      // of `in` (and `out`): IO_*
+  int dtype;           // of `in` (and `out`): IO_*
+  int large;           // which lists hold tiles of 128: 1 gram, 2 poly, 4 full
   const void* in;      // the matrices, or their gradients
   void* out;           // orthogonalised matrices (null: parameter update)
   float* buf;          // momentum (null: none)
@@ -219,9 +220,6 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(NsArgs p) {
 
 // ---------------------------------------------------------------- products
 #define NS_BK 32
-#ifndef NS_STAGES128
-#define NS_STAGES128 2
-#endif
 
 // Tiles in LDS.  k contiguous: T rows of 128 bytes, 16-byte chunk plane * 4 + k / 8 at slot chunk ^ ns_swz(row): 16 rows
 // reading the same chunk touch every bank once.
@@ -251,7 +249,7 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
                                            f32x16 (&acc)[T / 64][T / 64]) {
   constexpr int OPER = T * NS_BK * 4;         // bytes of an operand's k-tile, both planes
   constexpr int STAGE = 2 * OPER;
-  constexpr int NST = T == 128 ? NS_STAGES128 : 4;
+  constexpr int NST = T == 128 ? 2 : 3;
   constexpr int LPS = OPER / 2048;            // LDS-DMA instructions per wave and k-tile
   constexpr int MT = T / 64;
   const int lane = threadIdx.x & 63;
@@ -397,8 +395,11 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
 
 // fp32 tile in LDS: 16-byte writes of 8 rows at a time hit every bank once at this pitch
 #define NS_PITCH(T) ((T) + 4)
-#define NS_LDS_BYTES (NS_STAGES128 == 2 ? 128 * NS_PITCH(128) * 4 : NS_STAGES128 * 32768)
-static_assert(NS_LDS_BYTES >= NS_STAGES128 * 4 * 128 * NS_BK * 2 && NS_LDS_BYTES >= 4 * 4 * 64 * NS_BK * 2, "stages fit");
+// LDS of a launch with large tiles (two workgroups to a CU), and of one without (three)
+#define NS_LDS_LARGE (128 * NS_PITCH(128) * 4)
+#define NS_LDS_SMALL (3 * 4 * 64 * NS_BK * 2)
+static_assert(NS_LDS_LARGE >= 2 * 4 * 128 * NS_BK * 2 && NS_LDS_LARGE >= NS_LDS_SMALL, "stages fit");
+static_assert(NS_LDS_SMALL >= 64 * NS_PITCH(64) * 4, "the fp32 tile fits");
 
 // accumulators -> the tile [i][j] in LDS
 template <int T>
@@ -784,7 +785,7 @@ __global__ __launch_bounds__(256) void ns_small_kernel(NsArgs p, int k) {
     f32x4 v[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) v[n] = *(const f32x4*)(slab + n * 1024);
-#pragma unroll 2
+#pragma unroll 4
     for (int q = 1; q < job.k0; ++q)
 #pragma unroll
       for (int n = 0; n < 4; ++n) v[n] += *(const f32x4*)(slab + (size_t)q * 4096 + n * 1024);
@@ -857,18 +858,18 @@ __global__ __launch_bounds__(256) void ns_small_kernel(NsArgs p, int k) {
 
 // ---------------------------------------------------------------- host
 template <void (*KERNEL)(NsArgs, int)>
-static int ns_tiles(int blocks, const NsArgs& a, int k, hipStream_t st) {
+static int ns_tiles(int blocks, bool large, const NsArgs& a, int k, hipStream_t st) {
   // the dynamic-LDS limit is a per-device function attribute: remembered per device
   static bool attr_set[64] = {};
   int dev = 0;
   (void)hipGetDevice(&dev);
   dev = (dev >= 0 && dev < 64) ? dev : 0;
   if (!attr_set[dev]) {
-    const int rc = (int)hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, NS_LDS_BYTES);
+    const int rc = (int)hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, NS_LDS_LARGE);
     if (rc != 0) return rc;
     attr_set[dev] = true;
   }
-  hipLaunchKernelGGL(KERNEL, dim3(blocks), dim3(256), NS_LDS_BYTES, st, a, k);
+  hipLaunchKernelGGL(KERNEL, dim3(blocks), dim3(256), large ? NS_LDS_LARGE : NS_LDS_SMALL, st, a, k);
   return (int)hipGetLastError();
 }
 
@@ -891,7 +892,7 @@ static int ns_first(const NsArgs& a, hipStream_t st) {
 // the advancing stage of iteration k
 template <int WHAT, typename O>
 static int ns_step(const NsArgs& a, int k, hipStream_t st) {
-  if (a.nsmall == 0) return ns_tiles<ns_advance_kernel<WHAT, O>>(a.nfull, a, k, st);
+  if (a.nsmall == 0) return ns_tiles<ns_advance_kernel<WHAT, O>>(a.nfull, (a.large & 4) != 0, a, k, st);
   hipLaunchKernelGGL((ns_small_kernel<WHAT, O>), dim3(a.nsmall), dim3(256), 0, st, a, k);
   return (int)hipGetLastError();
 }
@@ -913,9 +914,9 @@ extern "C" int dtfa_newton_schulz(const NsArgs* args, hipStream_t st) {
          : ns_first<float, false>(a, st);
   for (int k = 0; k < a.steps && rc == 0; ++k) {
     if (a.nsmall == 0) {
-      rc = ns_tiles<ns_symmetric_kernel<false>>(a.ngram, a, k, st);
+      rc = ns_tiles<ns_symmetric_kernel<false>>(a.ngram, (a.large & 1) != 0, a, k, st);
       if (rc == 0 && a.ngram_joins > 0) rc = ns_join<false>(a.ngram_joins, a, k, st);
-      if (rc == 0) rc = ns_tiles<ns_symmetric_kernel<true>>(a.npoly, a, k, st);
+      if (rc == 0) rc = ns_tiles<ns_symmetric_kernel<true>>(a.npoly, (a.large & 2) != 0, a, k, st);
       if (rc == 0 && a.npoly_joins > 0) rc = ns_join<true>(a.npoly_joins, a, k, st);
       if (rc != 0) break;
     }

@@ -34,9 +34,9 @@ SLOTS = 2 * CUS           # workgroups at a time
 MIN_STEPS = 8             # shortest piece of a cut reduction
 
 # Shorter sides of at most 64 take one launch an iteration, in which every workgroup adds up the partial products of all
-# slices of its matrix (0.35 us each) and advances the 64 x 64 blocks of its own (1.2 us each): the time is least
-# at sqrt(1.2 / 0.35 * blocks) slices, and beyond 128 blocks the separate stages are faster.
-SMALL_BLOCKS_PER_SLICE2 = 1.2 / 0.35
+# slices of its matrix (about 0.25 us each) and advances the 64 x 64 blocks of its own (about 2.5 us each): the time is
+# least at sqrt(10 * blocks) slices.  64 x 576 fp32: 46 us against 80 in separate stages, 64 x 4608: 81 against 108.
+SMALL_BLOCKS_PER_SLICE2 = 10.0
 SMALL_MAX_LONG = 8192
 
 _MAT = np.dtype([("at", "<i8"), ("x", "<i8"), ("a", "<i8"), ("part", "<i8"), ("rows", "<i4"), ("cols", "<i4"),
@@ -49,7 +49,7 @@ class NsArgs(C.Structure):
                 ("poly", C.c_void_p), ("poly_joins", C.c_void_p), ("full", C.c_void_p), ("small", C.c_void_p), ("nsmall", C.c_int),
                 ("small_slices", C.c_int), ("nchunks", C.c_int),
                 ("npacks", C.c_int), ("ngram", C.c_int), ("ngram_joins", C.c_int), ("npoly", C.c_int),
-                ("npoly_joins", C.c_int), ("nfull", C.c_int), ("steps", C.c_int), ("dtype", C.c_int), ("pad", C.c_int), ("in_", C.c_void_p), ("out", C.c_void_p), ("buf", C.c_void_p),
+                ("npoly_joins", C.c_int), ("nfull", C.c_int), ("steps", C.c_int), ("dtype", C.c_int), ("large", C.c_int), ("in_", C.c_void_p), ("out", C.c_void_p), ("buf", C.c_void_p),
                 ("w", C.c_void_p), ("w16", C.c_void_p), ("hyper", C.c_void_p), ("part", C.c_void_p), ("slabs", C.c_void_p), ("ws", C.c_void_p), ("nparts", C.c_longlong),
                 ("eps", C.c_float), ("mu", C.c_float), ("wd", C.c_float), ("nesterov", C.c_int)]
 
@@ -249,6 +249,7 @@ class NsPlan:
                  _join(poly_joins), _over_xcds(full), _join(small)]
         counts = [len(v) for v in lists]
         self.counts = [counts[7], small_slices] + counts[:7]
+        self.large = sum(bit for bit, at in ((1, 2), (2, 4), (4, 6)) if (lists[at][:, 3] == 128).any())
         # 32-byte aligned: the lists are read 16 and 32 bytes at a time
         blobs = [v.tobytes() + b"\0" * (-v.nbytes % 32) for v in [mats] + lists]
         self.table = torch.from_numpy(np.frombuffer(b"".join(blobs), dtype=np.uint8).copy()).to(device)
@@ -263,7 +264,7 @@ class NsPlan:
             ws = torch.empty(self.ws_elems, dtype=torch.float16, device=dev)
             part = torch.empty(self.parts + self.mats, dtype=torch.float64, device=dev)
             slabs = torch.empty(self.slabs * 4096, dtype=F32, device=dev) if self.slabs else None
-            args = NsArgs(*self.places, *self.counts, steps, DTYPES[inp.dtype], 0, inp.data_ptr(), hipk.ptr(out), hipk.ptr(buf),
+            args = NsArgs(*self.places, *self.counts, steps, DTYPES[inp.dtype], self.large, inp.data_ptr(), hipk.ptr(out), hipk.ptr(buf),
                           hipk.ptr(w), hipk.ptr(w16), hipk.ptr(hyper), part.data_ptr(), hipk.ptr(slabs), ws.data_ptr(),
                           self.parts, NORM_EPS, mu, wd, 1 if nesterov else 0)
             hipk.check(hipk.lib().dtfa_newton_schulz(C.byref(args), hipk.stream()), "newton_schulz")
