@@ -14,18 +14,23 @@ import torch
 import torch.nn as nn
 
 from ..ops import functional as F
-from .layers import ConvBnAct, Dense
+from .layers import ConvBnAct, Dense, LayerNorm
 
 IMAGE_CHANNELS = 8
+HEAD_NORM_SCOPE = "fc_trainable/feature_norm"
 
 
 class FlowerHead(nn.Module):
     """dense(1024, relu) -> dropout(rate) -> dense(n_outputs) with the optional
     L2 *activity* regulariser of the reference (scale 0.0005 on both dense
-    outputs; recognition_flower/single/flower_train.py:71,77,84)."""
+    outputs; recognition_flower/single/flower_train.py:71,77,84).  ``norm="layer"`` layer-normalises the features first, so
+    that the head sees them at one scale whatever the trunk's statistics are (``norm="none"``: the reference's head)."""
 
-    def __init__(self, n_in, n_outputs=5, hidden=1024, dropout_rate=0.5, act_l2=0.0005):
+    def __init__(self, n_in, n_outputs=5, hidden=1024, dropout_rate=0.5, act_l2=0.0005, norm="none"):
         super().__init__()
+        if norm not in ("none", "layer"):
+            raise ValueError("head norm must be 'none' or 'layer', got %r" % (norm,))
+        self.feature_norm = LayerNorm(n_in, tf_scope=HEAD_NORM_SCOPE) if norm == "layer" else None
         self.n_outputs = n_outputs
         self.dropout_rate = dropout_rate
         self.act_l2 = act_l2
@@ -33,6 +38,8 @@ class FlowerHead(nn.Module):
         self.flower_logits = Dense(hidden, n_outputs, tf_scope="fc_trainable/flower_logits")
 
     def forward(self, feats):
+        if self.feature_norm is not None:
+            feats = self.feature_norm(feats)
         h = self.dense_prelogit1(feats)
         reg = None
         if self.act_l2:
@@ -43,7 +50,7 @@ class FlowerHead(nn.Module):
 
 
 class FlowerCNN(nn.Module):
-    def __init__(self, num_classes=5, widths=(32, 64, 128, 256, 512), dropout_rate=0.5, act_l2=0.0005):
+    def __init__(self, num_classes=5, widths=(32, 64, 128, 256, 512), dropout_rate=0.5, act_l2=0.0005, head_norm="none"):
         super().__init__()
         self.num_classes = num_classes
         w = widths
@@ -52,7 +59,7 @@ class FlowerCNN(nn.Module):
         self.conv3 = ConvBnAct(w[1], w[2], 3, 1, "SAME", tf_scope="FlowerCNN/conv3")
         self.conv4 = ConvBnAct(w[2], w[3], 3, 1, "SAME", tf_scope="FlowerCNN/conv4")
         self.conv5 = ConvBnAct(w[3], w[4], 3, 1, "SAME", tf_scope="FlowerCNN/conv5")
-        self.head = FlowerHead(w[4], num_classes, dropout_rate=dropout_rate, act_l2=act_l2)
+        self.head = FlowerHead(w[4], num_classes, dropout_rate=dropout_rate, act_l2=act_l2, norm=head_norm)
 
     def features(self, x):
         x = self.conv1(x)

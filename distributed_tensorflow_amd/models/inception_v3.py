@@ -279,7 +279,8 @@ class InceptionV3Flower(nn.Module):
     ``AuxLogits`` / ``Logits``, which no loss touches, stay frozen.
     """
 
-    def __init__(self, num_classes=5, head_dropout_rate=0.5, act_l2=0.0005, trunk_bn="batch", train_trunk=False):
+    def __init__(self, num_classes=5, head_dropout_rate=0.5, act_l2=0.0005, trunk_bn="batch", train_trunk=False,
+                 head_norm="none"):
         super().__init__()
         if trunk_bn not in ("batch", "moving"):
             raise ValueError("trunk_bn must be 'batch' or 'moving'")
@@ -291,7 +292,7 @@ class InceptionV3Flower(nn.Module):
                   for p in getattr(self.trunk, name).parameters()}
         for p in self.trunk.parameters():
             p.requires_grad_(self.train_trunk and id(p) not in unused)
-        self.head = FlowerHead(2048, num_classes, dropout_rate=head_dropout_rate, act_l2=act_l2)
+        self.head = FlowerHead(2048, num_classes, dropout_rate=head_dropout_rate, act_l2=act_l2, norm=head_norm)
 
     def train(self, mode: bool = True):
         super().train(mode)

@@ -467,6 +467,9 @@ class PSWorkerEngine:
         so the worker runs at max(device time, network time) per step instead of their sum."""
         from .flat import FlatParams
 
+        if optimizer.lower() not in ("adam", "momentum", "sgd"):
+            # (said here: the ps task, which runs the optimizer, would only find out once the chief initialises it)
+            raise ValueError("parameter-server tasks run adam or momentum, not %r" % optimizer)
         self.model = model
         self.worker_index = worker_index
         self.is_chief = is_chief

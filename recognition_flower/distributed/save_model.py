@@ -56,6 +56,7 @@ def main(argv):
     from distributed_tensorflow_amd.io.export import export_servable
     from distributed_tensorflow_amd.io.saver import Saver
     from distributed_tensorflow_amd.models import build_model
+    from distributed_tensorflow_amd.models.flower_cnn import HEAD_NORM_SCOPE
 
     device = FLAGS.device
     if device == "auto":
@@ -63,9 +64,12 @@ def main(argv):
     device = torch.device(device)
     flower_classes = load_classes()
     model_name = FLAGS.model if FLAGS.model != "auto" else ("inception_v3_head" if device.type == "cuda" else "flower_cnn")
-    model = build_model(model_name, num_classes=len(flower_classes), device=device)
-    saver = Saver(model)
     ckpt = bundle.latest_checkpoint(FLAGS.checkpoint_dir)
+    # (a head with a feature norm is known by its variables)
+    names = {entry[0] for entry in bundle.list_bundle(ckpt)} if ckpt is not None else set()
+    model_kwargs = {"head_norm": "layer"} if HEAD_NORM_SCOPE + "/gamma" in names else {}
+    model = build_model(model_name, num_classes=len(flower_classes), device=device, **model_kwargs)
+    saver = Saver(model)
     step = 0
     if ckpt is not None:
         step = saver.restore(ckpt, restore_slots=False)
@@ -80,7 +84,7 @@ def main(argv):
         logits = out[0] if isinstance(out, tuple) else out
         print("smoke logits:", logits[0, :len(flower_classes)].float().tolist())
     path = export_servable(model, flower_classes, FLAGS.output_dir, FLAGS.model_version, model_name=model_name,
-                           image_size=FLAGS.image_size, global_step=step)
+                           image_size=FLAGS.image_size, model_kwargs=model_kwargs, global_step=step)
     print("Exported servable to", path)
     print("Done exporting!")
     return 0

@@ -85,9 +85,13 @@ flags.DEFINE_string("ps_apply", "auto", "ps_backend=xgmi: per_push (one optimize
                     "aggregate (staleness 0 only: one step per round on the sum of the workers' gradients) | auto")
 flags.DEFINE_string("ps_pipeline", "auto", "ps_backend=tcp: push and pull on a helper thread while the device computes the next step (one "
                     "more step of staleness on the worker's own gradient) -- true | false | auto (on unless --staleness=0)")
-flags.DEFINE_string("optimizer", "adam", "adam (the reference) | momentum")
-flags.DEFINE_float("momentum", 0.9, "momentum optimizer: heavy-ball coefficient.")
-flags.DEFINE_float("weight_decay", 0.0, "momentum optimizer: L2 weight decay on convolution / dense kernels.")
+flags.DEFINE_string("optimizer", "adam", "adam (the reference) | momentum | muon (orthogonalised momentum on convolution / dense "
+                    "kernels, Adam on the rest; --mode=sync_dp or async_ssp, --learning_rate around 0.02)")
+flags.DEFINE_float("momentum", 0.9, "momentum and muon optimizers: heavy-ball coefficient.")
+flags.DEFINE_float("weight_decay", 0.0, "momentum optimizer: L2 weight decay on convolution / dense kernels; muon: decoupled "
+                   "weight decay on them.")
+flags.DEFINE_string("head_norm", "none", "none (the reference) | layer: layer-normalise the features in front of the flower head; "
+                    "the same on every task.")
 flags.DEFINE_integer("lr_decay_steps", 0, "Exponential learning-rate decay period in global steps (0 = constant rate, as "
                      "the reference's distributed script; its single-process script uses 200).")
 flags.DEFINE_float("lr_decay_rate", 0.95, "Exponential learning-rate decay factor per lr_decay_steps.")
@@ -135,10 +139,21 @@ def train_input_fn(tfrecords_path, params, device, rank, world, channels=8):
                        channels=channels)
 
 
+def _head_kwargs(model_name):
+    if FLAGS.head_norm == "none":
+        return {}
+    if model_name == "resnet50":
+        raise ValueError("--head_norm=%s: %s has no flower head" % (FLAGS.head_norm, model_name))
+    return {"head_norm": FLAGS.head_norm}
+
+
 def _optimizer_config():
     """(optimizer name, its keyword arguments, learning rate or schedule) from the flags; the same on every task."""
     name = FLAGS.optimizer.lower()
-    kwargs = {"momentum": FLAGS.momentum, "weight_decay": FLAGS.weight_decay} if name == "momentum" else {}
+    kwargs = {"momentum": FLAGS.momentum, "weight_decay": FLAGS.weight_decay} if name in ("momentum", "muon") else {}
+    if name == "muon" and FLAGS.mode not in ("sync_dp", "async_ssp"):
+        raise ValueError("--optimizer=muon needs whole matrices on every worker: --mode=sync_dp or --mode=async_ssp, not %s"
+                         % FLAGS.mode)
     rate = params["learning_rate"]
     if FLAGS.lr_decay_steps > 0:
         from distributed_tensorflow_amd.optim.schedules import exponential_decay
@@ -226,7 +241,8 @@ def run_worker(spec):
         kw = {"head_dropout_rate": FLAGS.head_dropout_rate, "trunk_bn": FLAGS.trunk_bn}
     else:
         kw = {"dropout_rate": FLAGS.head_dropout_rate} if model_name == "flower_cnn" else {}
-    model = build_model(model_name, num_classes=n_classes, device=device, **kw)
+    opt_name, opt_kwargs, lr_schedule = _optimizer_config()
+    model = build_model(model_name, num_classes=n_classes, device=device, **kw, **_head_kwargs(model_name))
     if FLAGS.bn_decay > 0 and hasattr(model, "trunk"):
         from distributed_tensorflow_amd.models.layers import ConvBnAct
 
@@ -234,7 +250,6 @@ def run_worker(spec):
             if isinstance(m, ConvBnAct):
                 m.momentum = 1.0 - FLAGS.bn_decay
 
-    opt_name, opt_kwargs, lr_schedule = _optimizer_config()
     lr = params["learning_rate"]
     xgmi = FLAGS.mode == "async_ps" and FLAGS.ps_backend == "xgmi"
     if xgmi:
@@ -381,7 +396,7 @@ def run_evaluator(spec):
     device = _device()
     model_name = _model_name(device)
     n_classes = _num_classes()
-    model = build_model(model_name, num_classes=n_classes, device=device).eval()
+    model = build_model(model_name, num_classes=n_classes, device=device, **_head_kwargs(model_name)).eval()
     saver = Saver(model)
     writer = EventWriter(os.path.join(FLAGS.summaries_dir + str(FLAGS.model_version), "eval"))
     eval_params = dict(params, num_epochs=1)
@@ -432,6 +447,7 @@ def main(unused_argv):
 
     print(os.environ.get("TF_CONFIG"))
     spec = parse_tf_config()
+    _optimizer_config()  # (a combination that cannot run ends every task at once, none waits for the others)
     if spec.task_type == "ps":
         return run_ps(spec)
     if spec.task_type == "evaluator":

@@ -376,3 +376,31 @@ def test_model_trains_with_muon_and_matches_the_cpu():
             assert (got - want).norm().item() <= _allowed(u, want) + slack, (r, c)
         for at, n in region.vectors:
             assert moved[at:at + n].abs().max().item() > 0
+
+
+@pytest.mark.parametrize("mode,kw", [("sync_dp", {}), ("async_ssp", {"staleness": 1})])
+def test_step_graph_with_a_normalised_head_matches_eager(mode, kw):
+    # layer normalisation, its gradients into the flat buffers and the Muon step together, eager and replayed
+    from distributed_tensorflow_amd.train.session import TrainingSession
+
+    def run(hip_graph):
+        torch.manual_seed(9)
+        model = build_model("flower_cnn", 5, device="cuda", dropout_rate=0.0, head_norm="layer")
+        eng = DataParallelEngine(model, mode=mode, optimizer="muon", lr=lambda t: 0.02 / (1 + t), opt_kwargs={"weight_decay": 0.01},
+                                 **kw)
+        sess = TrainingSession(model, eng, num_classes=5, hip_graph=hip_graph, graph_warmup_steps=2)
+        gen = torch.Generator().manual_seed(4)
+        losses = []
+        for _ in range(6):
+            x = torch.zeros(8, 64, 64, 8)
+            x[..., :3] = torch.rand(8, 64, 64, 3, generator=gen) * 2 - 1
+            y = torch.randint(0, 5, (8,), generator=gen, dtype=torch.int32)
+            losses.append(sess.run_step(x.cuda().bfloat16(), y.cuda()).loss)
+        assert (sess._graph is not None) == (hip_graph and eng.graph_capturable)
+        assert not torch.equal(model.head.feature_norm.gamma, torch.ones_like(model.head.feature_norm.gamma))
+        return losses, [g.master.clone() for g in eng.flat.groups]
+
+    (l0, w0), (l1, w1) = run(False), run(True)
+    assert l0 == l1 and all(math.isfinite(l) for l in l0)
+    for a, b in zip(w0, w1):
+        assert torch.equal(a, b)

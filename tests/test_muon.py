@@ -267,3 +267,39 @@ def test_checkpoint_round_trip(tmp_path):
     train(other, engine2, 1)
     for (n, p), q in zip(model.named_parameters(), other.parameters()):
         assert torch.equal(p, q), n
+
+
+def test_head_with_feature_norm_trains_and_exports_under_its_own_names(tmp_path):
+    from distributed_tensorflow_amd.io.export import Servable, export_servable
+
+    torch.manual_seed(7)
+    kw = dict(widths=(8, 8, 16, 16, 24), dropout_rate=0.0, head_norm="layer")
+    model = build_model("flower_cnn", 5, **kw).train()
+    engine = DataParallelEngine(model, mode="sync_dp", optimizer="muon", lr=0.02)
+    saver = Saver(model, engine)
+    x = torch.zeros(4, 32, 32, 8)
+    x[..., :3] = torch.randn(4, 32, 32, 3, generator=torch.Generator().manual_seed(8))
+    for _ in range(2):
+        engine.begin_step()
+        logits, reg = model(x)
+        (F.softmax_xent(logits, torch.tensor([0, 1, 2, 3]), 5)[0] + reg).backward()
+        engine.finish_step()
+    assert not torch.equal(model.head.feature_norm.gamma, torch.ones(24))
+    names = saver.variables()
+    assert {"fc_trainable/feature_norm/gamma", "fc_trainable/feature_norm/beta/Adam",
+            "fc_trainable/dense_prelogit1/kernel/Momentum"} <= set(names)
+    path = export_servable(model, list("abcde"), str(tmp_path), 1, model_name="flower_cnn", image_size=32, model_kwargs=kw,
+                           engine=engine)
+    served = Servable(path, device="cpu").model
+    model.eval()
+    with torch.no_grad():
+        torch.testing.assert_close(served(x)[0], model(x)[0], rtol=1e-5, atol=1e-5)
+    with pytest.raises(ValueError):
+        build_model("flower_cnn", 5, head_norm="batch")
+
+
+def test_parameter_servers_refuse_muon():
+    from distributed_tensorflow_amd.parallel.ps import PSWorkerEngine
+
+    with pytest.raises(ValueError, match="muon"):
+        PSWorkerEngine(_model(), [("127.0.0.1", 1)], 0, True, optimizer="muon")
