@@ -214,8 +214,9 @@ struct LnBwd {
   int cols;
 };
 
+// (`block` of `blocks` workgroups)
 template <typename T, int TPR, int NV, bool PARAMS>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV == 1 ? 4 : NV == 2 ? 3 : 2) void layer_norm_bwd_kernel(LnBwd p) {
+__device__ __forceinline__ void ln_bwd_rows(const LnBwd& p, unsigned block, unsigned blocks) {
   typedef typename RowVec<T>::V V;
   constexpr int VEC = RowVec<T>::N;
   constexpr int BLOCK = TPR < 256 ? 256 : TPR;
@@ -275,8 +276,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV == 1 ? 4 : NV == 2 ? 3 : 
       f.rstd = p.rstd[row];
     }
   };
-  const long long stride = (long long)gridDim.x * RPB;
-  long long base = (long long)blockIdx.x * RPB;
+  const long long stride = (long long)blocks * RPB;
+  long long base = (long long)block * RPB;
   Row r, next;
   if (base < p.rows) fetch(base, r);
   for (; base < p.rows; base += stride) {
@@ -340,7 +341,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV == 1 ? 4 : NV == 2 ? 3 : 
   }
   if (!PARAMS) return;
   // threads of one column position in the rows side by side: lanes TPR apart, then the waves of the workgroup
-  float* pg = p.part + (size_t)blockIdx.x * 2 * p.cols;
+  float* pg = p.part + (size_t)block * 2 * p.cols;
   float* pb = pg + p.cols;
 #pragma unroll
   for (int off = 32; off >= TPR; off >>= 1) {
@@ -396,6 +397,68 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV == 1 ? 4 : NV == 2 ? 3 : 
       pb[whole + t] = abe;
     }
   }
+}
+
+template <typename T, int TPR, int NV, bool PARAMS>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV == 1 ? 4 : NV == 2 ? 3 : 2) void layer_norm_bwd_kernel(LnBwd p) {
+  ln_bwd_rows<T, TPR, NV, PARAMS>(p, blockIdx.x, gridDim.x);
+}
+
+// dgamma / dbeta of a strip of columns, over all rows: 8 threads side by side, a vector of columns each, and 32 row lanes,
+// added up in a fixed order.
+template <typename T>
+__device__ __forceinline__ void ln_bwd_strip(const LnBwd& p, unsigned strip, float* dgamma, float* dbeta) {
+  constexpr int VEC = RowVec<T>::N;
+  __shared__ float meet[4][2][8 * VEC];
+  const int cl = threadIdx.x & 7, rl = threadIdx.x >> 3, wave = threadIdx.x >> 6;
+  const int col = (int)(strip * 8 + cl) * VEC;
+  float ag[VEC], ab[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) ag[j] = ab[j] = 0.f;
+  if (col < p.cols)
+#pragma unroll 4
+    for (long long row = rl; row < p.rows; row += 32) {
+      float x[VEC], d[VEC];
+      row_load<T, VEC>((const T*)p.x + row * p.ldx, col, p.cols, x);
+      row_load<T, VEC>((const T*)p.dy + row * p.lddy, col, p.cols, d);
+      const float mean = p.mean[row], rstd = p.rstd[row];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        ag[j] += d[j] * ((x[j] - mean) * rstd);
+        ab[j] += d[j];
+      }
+    }
+#pragma unroll
+  for (int off = 8; off < 64; off <<= 1)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      ag[j] += __shfl_xor(ag[j], off, 64);
+      ab[j] += __shfl_xor(ab[j], off, 64);
+    }
+  if ((threadIdx.x & 63) < 8)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      meet[wave][0][cl * VEC + j] = ag[j];
+      meet[wave][1][cl * VEC + j] = ab[j];
+    }
+  __syncthreads();
+  for (int e = threadIdx.x; e < 16 * VEC; e += 256) {
+    const int which = e / (8 * VEC), c = e % (8 * VEC), at = (int)strip * 8 * VEC + c;
+    float* out = which ? dbeta : dgamma;
+    if (out != nullptr && at < p.cols)
+      out[at] = (meet[0][which][c] + meet[1][which][c]) + (meet[2][which][c] + meet[3][which][c]);
+  }
+}
+
+// Few rows: the whole backward pass in one launch.  The row statistics are known, so dgamma and dbeta need nothing of dx:
+// workgroups beyond the first `blocks` take strips of columns and read x and dy once more, from the L2.  (At these sizes a
+// launch costs more than the bytes: 256 x 2048 bf16 is 2 MB.)
+template <typename T, int TPR, int NV>
+__global__ __launch_bounds__(256) void layer_norm_bwd_few_kernel(LnBwd p, unsigned blocks, float* dgamma, float* dbeta) {
+  if (blockIdx.x < blocks)
+    ln_bwd_rows<T, TPR, NV, false>(p, blockIdx.x, blocks);
+  else
+    ln_bwd_strip<T>(p, blockIdx.x - blocks, dgamma, dbeta);
 }
 
 // [parts][2][cols] -> dgamma, dbeta.  32 columns x 32 row lanes: lane r sums parts r, r + 32, ... and the lanes are
@@ -571,8 +634,11 @@ extern "C" int dtfa_layer_norm_fwd(const void* x, long long ldx, const float* ga
   return -2;
 }
 
-// Workgroups (= partial rows) of the backward pass: what stays resident on 256 CUs, no more than there are rows for.
+// Partial rows that the backward pass wants scratch for (= its workgroups: what stays resident on 256 CUs, no more than
+// there are rows for); 0 where it takes none.
+static bool ln_few(long long rows, int cols, int dtype);
 extern "C" int dtfa_layer_norm_bwd_parts(long long rows, int cols, int dtype) {
+  if (ln_few(rows, cols, dtype)) return 0;
   const long long nvec = ln_vectors(cols, dtype);
   const int tpr = nvec <= 8 ? 8 : nvec <= 16 ? 16 : nvec <= 24 ? 8 : nvec <= 32 ? 32 : nvec <= 48 ? 16 : nvec <= 64 ? 64
                   : nvec <= 96 ? 32 : nvec <= 256 ? 64 : nvec <= 512 ? 128 : 256;
@@ -587,9 +653,26 @@ extern "C" int dtfa_layer_norm_bwd_parts(long long rows, int cols, int dtype) {
   return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
+// one launch for everything
+#define LN_FEW_ROWS 1024
+#define LN_FEW_ELEMENTS (1 << 21)
+static bool ln_few(long long rows, int cols, int dtype) {
+  return rows <= LN_FEW_ROWS && rows * cols <= LN_FEW_ELEMENTS && ln_vectors(cols, dtype) <= 1024;
+}
+
 template <typename T, int TPR, int NV>
-static int ln_bwd_launch(const LnBwd& p, int parts, hipStream_t st) {
+static int ln_bwd_launch(const LnBwd& p, int parts, float* dgamma, float* dbeta, hipStream_t st) {
   constexpr int BLOCK = TPR < 256 ? 256 : TPR;
+  if constexpr (BLOCK == 256) {
+    if (p.part == nullptr && (dgamma != nullptr || dbeta != nullptr)) {
+      constexpr int RPB = BLOCK / TPR, COLS = 8 * RowVec<T>::N;
+      const unsigned blocks = p.dx != nullptr ? (unsigned)((p.rows + RPB - 1) / RPB) : 0;
+      const unsigned strips = (unsigned)((p.cols + COLS - 1) / COLS);
+      hipLaunchKernelGGL((layer_norm_bwd_few_kernel<T, TPR, NV>), dim3(blocks + strips), dim3(256), 0, st, p, blocks, dgamma,
+                         dbeta);
+      return (int)hipGetLastError();
+    }
+  }
   if (p.part != nullptr)
     hipLaunchKernelGGL((layer_norm_bwd_kernel<T, TPR, NV, true>), dim3(parts), dim3(BLOCK), 0, st, p);
   else
@@ -598,20 +681,20 @@ static int ln_bwd_launch(const LnBwd& p, int parts, hipStream_t st) {
 }
 
 template <typename T>
-static int ln_bwd(const LnBwd& p, long long nvec, int parts, hipStream_t st) {
-  if (nvec <= 8) return ln_bwd_launch<T, 8, 1>(p, parts, st);
-  if (nvec <= 16) return ln_bwd_launch<T, 16, 1>(p, parts, st);
-  if (nvec <= 24) return ln_bwd_launch<T, 8, 3>(p, parts, st);
-  if (nvec <= 32) return ln_bwd_launch<T, 32, 1>(p, parts, st);
-  if (nvec <= 48) return ln_bwd_launch<T, 16, 3>(p, parts, st);
-  if (nvec <= 64) return ln_bwd_launch<T, 64, 1>(p, parts, st);
-  if (nvec <= 96) return ln_bwd_launch<T, 32, 3>(p, parts, st);
-  if (nvec <= 128) return ln_bwd_launch<T, 64, 2>(p, parts, st);
-  if (nvec <= 192) return ln_bwd_launch<T, 64, 3>(p, parts, st);
-  if (nvec <= 256) return ln_bwd_launch<T, 64, 4>(p, parts, st);
-  if (nvec <= 512) return ln_bwd_launch<T, 128, 4>(p, parts, st);
-  if (nvec <= 1024) return ln_bwd_launch<T, 256, 4>(p, parts, st);
-  if (nvec <= 2048) return ln_bwd_launch<T, 512, 4>(p, parts, st);
+static int ln_bwd(const LnBwd& p, long long nvec, int parts, float* dgamma, float* dbeta, hipStream_t st) {
+  if (nvec <= 8) return ln_bwd_launch<T, 8, 1>(p, parts, dgamma, dbeta, st);
+  if (nvec <= 16) return ln_bwd_launch<T, 16, 1>(p, parts, dgamma, dbeta, st);
+  if (nvec <= 24) return ln_bwd_launch<T, 8, 3>(p, parts, dgamma, dbeta, st);
+  if (nvec <= 32) return ln_bwd_launch<T, 32, 1>(p, parts, dgamma, dbeta, st);
+  if (nvec <= 48) return ln_bwd_launch<T, 16, 3>(p, parts, dgamma, dbeta, st);
+  if (nvec <= 64) return ln_bwd_launch<T, 64, 1>(p, parts, dgamma, dbeta, st);
+  if (nvec <= 96) return ln_bwd_launch<T, 32, 3>(p, parts, dgamma, dbeta, st);
+  if (nvec <= 128) return ln_bwd_launch<T, 64, 2>(p, parts, dgamma, dbeta, st);
+  if (nvec <= 192) return ln_bwd_launch<T, 64, 3>(p, parts, dgamma, dbeta, st);
+  if (nvec <= 256) return ln_bwd_launch<T, 64, 4>(p, parts, dgamma, dbeta, st);
+  if (nvec <= 512) return ln_bwd_launch<T, 128, 4>(p, parts, dgamma, dbeta, st);
+  if (nvec <= 1024) return ln_bwd_launch<T, 256, 4>(p, parts, dgamma, dbeta, st);
+  if (nvec <= 2048) return ln_bwd_launch<T, 512, 4>(p, parts, dgamma, dbeta, st);
   if (p.dx != nullptr) {
     const long long grid = p.rows < LN_MAX_GRID ? p.rows : LN_MAX_GRID;
     hipLaunchKernelGGL((layer_norm_dx_long_kernel<T>), dim3((unsigned)grid), dim3(1024), 0, st, p);
@@ -623,19 +706,22 @@ static int ln_bwd(const LnBwd& p, long long nvec, int parts, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
-// `part`: [dtfa_layer_norm_bwd_parts()][2][cols] fp32 scratch, null when neither dgamma nor dbeta is wanted.
+// `part`: [dtfa_layer_norm_bwd_parts()][2][cols] fp32 scratch, null when that is 0 or neither dgamma nor dbeta is wanted.
 extern "C" int dtfa_layer_norm_bwd(const void* x, long long ldx, const void* dy, long long lddy, const float* gamma,
                                    const float* stats, void* dx, float* part, float* dgamma, float* dbeta, long long rows,
                                    int cols, int dtype, hipStream_t st) {
   if (cols <= 0 || rows <= 0 || ldx < 0 || lddy < 0) return -1;
-  if ((dgamma != nullptr || dbeta != nullptr) != (part != nullptr)) return -1;
-  if (dx == nullptr && part == nullptr) return 0;
+  const bool params = dgamma != nullptr || dbeta != nullptr;
+  const int parts = dtfa_layer_norm_bwd_parts(rows, cols, dtype);
+  if ((params && parts > 0) != (part != nullptr)) return -1;
+  if (dx == nullptr && !params) return 0;
   const LnBwd p = {x, ldx, dy, lddy, gamma, stats, stats + rows, dx, part, rows, cols};
   const long long nvec = ln_vectors(cols, dtype);
-  const int parts = dtfa_layer_norm_bwd_parts(rows, cols, dtype);
-  int rc = dtype == IO_BF16 ? ln_bwd<bf16>(p, nvec, parts, st)
-           : dtype == IO_F16 ? ln_bwd<f16>(p, nvec, parts, st)
-           : dtype == IO_F32 ? ln_bwd<float>(p, nvec, parts, st) : -2;
+  // (without sums of columns the grid is what the sums' would be)
+  const int grid = parts > 0 ? parts : (int)(rows < 1024 ? rows : 1024);
+  int rc = dtype == IO_BF16 ? ln_bwd<bf16>(p, nvec, grid, dgamma, dbeta, st)
+           : dtype == IO_F16 ? ln_bwd<f16>(p, nvec, grid, dgamma, dbeta, st)
+           : dtype == IO_F32 ? ln_bwd<float>(p, nvec, grid, dgamma, dbeta, st) : -2;
   if (rc != 0 || part == nullptr) return rc;
   hipLaunchKernelGGL(layer_norm_params_kernel, dim3((unsigned)((2LL * cols + 31) / 32)), dim3(1024), 0, st, part, parts,
                      cols, dgamma, dbeta);

@@ -617,9 +617,8 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, gamma: Optional[torch.Tens
         if rows:
             L, dt = hipk.lib(), _LN_DTYPES[x.dtype]
             (xr, ldx), (gr, ldg) = _ln_rows(x), _ln_rows(dy)
-            part = None
-            if want_dgamma or want_dbeta:
-                part = torch.empty(L.dtfa_layer_norm_bwd_parts(rows, cols, dt) * 2 * cols, dtype=F32, device=x.device)
+            parts = L.dtfa_layer_norm_bwd_parts(rows, cols, dt) if want_dgamma or want_dbeta else 0
+            part = torch.empty(parts * 2 * cols, dtype=F32, device=x.device) if parts else None
             hipk.check(L.dtfa_layer_norm_bwd(xr.data_ptr(), ldx, gr.data_ptr(), ldg, hipk.ptr(gamma), stats.data_ptr(),
                                              hipk.ptr(dx), hipk.ptr(part), hipk.ptr(dgamma), hipk.ptr(dbeta), rows, cols, dt, hipk.stream()), "layer_norm_bwd")
     return dx, dgamma, dbeta
