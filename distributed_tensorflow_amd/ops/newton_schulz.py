@@ -9,7 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import heapq
 import math
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -46,12 +46,13 @@ _MAT = np.dtype([("at", "<i8"), ("x", "<i8"), ("a", "<i8"), ("part", "<i8"), ("r
 
 
 class NsArgs(C.Structure):
-    _fields_ = [("mats", C.c_void_p), ("chunks", C.c_void_p), ("packs", C.c_void_p), ("gram", C.c_void_p), ("joins", C.c_void_p),
-                ("poly", C.c_void_p), ("poly_joins", C.c_void_p), ("full", C.c_void_p), ("small", C.c_void_p), ("nsmall", C.c_int),
-                ("small_slices", C.c_int), ("nchunks", C.c_int),
-                ("npacks", C.c_int), ("ngram", C.c_int), ("ngram_joins", C.c_int), ("npoly", C.c_int),
-                ("npoly_joins", C.c_int), ("nfull", C.c_int), ("steps", C.c_int), ("dtype", C.c_int), ("large", C.c_int), ("in_", C.c_void_p), ("out", C.c_void_p), ("buf", C.c_void_p),
-                ("w", C.c_void_p), ("w16", C.c_void_p), ("hyper", C.c_void_p), ("part", C.c_void_p), ("slabs", C.c_void_p), ("ws", C.c_void_p), ("nparts", C.c_longlong),
+    _fields_ = [("mats", C.c_void_p), ("chunks", C.c_void_p), ("packs", C.c_void_p), ("gram", C.c_void_p),
+                ("joins", C.c_void_p), ("poly", C.c_void_p), ("poly_joins", C.c_void_p), ("full", C.c_void_p),
+                ("small", C.c_void_p), ("nsmall", C.c_int), ("small_slices", C.c_int), ("nchunks", C.c_int),
+                ("npacks", C.c_int), ("ngram", C.c_int), ("ngram_joins", C.c_int), ("npoly", C.c_int), ("npoly_joins", C.c_int),
+                ("nfull", C.c_int), ("steps", C.c_int), ("dtype", C.c_int), ("large", C.c_int),
+                ("in_", C.c_void_p), ("out", C.c_void_p), ("buf", C.c_void_p), ("w", C.c_void_p), ("w16", C.c_void_p),
+                ("hyper", C.c_void_p), ("part", C.c_void_p), ("slabs", C.c_void_p), ("ws", C.c_void_p), ("nparts", C.c_longlong),
                 ("eps", C.c_float), ("mu", C.c_float), ("wd", C.c_float), ("nesterov", C.c_int)]
 
 
@@ -270,10 +271,17 @@ class NsPlan:
         starts = np.cumsum([0] + [len(v) for v in blobs])
         self.places = [self.table.data_ptr() + int(s) for s in starts[:9]]
         self.ws_elems, self.parts, self.mats, self.slabs = ws, part, len(matrices), slabs
+        self.first = min(at for at, _, _ in matrices)
+        self.end = max(at + rows * cols for at, rows, cols in matrices)
 
     def launch(self, *, inp: torch.Tensor, steps: int, out=None, buf=None, w=None, w16=None, hyper=None, mu=0.0,
                nesterov=False, wd=0.0) -> None:
         dev = inp.device
+        if dev != self.table.device:
+            raise ValueError("orthogonalize: a plan for %s cannot run on %s" % (self.table.device, dev))
+        if self.first < 0 or self.end > inp.numel():
+            raise ValueError("orthogonalize: the plan's matrices take the values %d .. %d of a buffer of %d"
+                             % (self.first, self.end, inp.numel()))
         with hipk.device_of(inp):
             ws = torch.empty(self.ws_elems, dtype=torch.float16, device=dev)
             part = torch.empty(self.parts + self.mats, dtype=torch.float64, device=dev)
@@ -287,16 +295,15 @@ class NsPlan:
 _plans: Dict[tuple, NsPlan] = {}
 
 
-def get_plan(matrices: Sequence[Tuple[int, int, int]], device: torch.device) -> NsPlan:
-    """The plan of these matrices on ``device``.  Plans stay for the life of the process, like those of the convolutions:
-    kernels in flight on any stream, and captured graphs, hold their addresses."""
-    key = (tuple(matrices), device.index)
-    plan = _plans.get(key)
+def get_plan(key: tuple, matrices: Callable[[], Sequence[Tuple[int, int, int]]], device: torch.device) -> NsPlan:
+    """The plan of the matrices that ``key`` stands for on ``device``.  Plans stay for the life of the process, like those of
+    the convolutions: kernels in flight on any stream, and captured graphs, hold their addresses."""
+    plan = _plans.get((key, device.index))
     if plan is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("orthogonalize: the first call of these shapes uploads their plan and cannot be captured: run "
                                "it once before the capture")
-        plan = _plans[key] = NsPlan(matrices, device)
+        plan = _plans.setdefault((key, device.index), NsPlan(matrices(), device))
     return plan
 
 
@@ -312,7 +319,7 @@ def orthogonalize(x: torch.Tensor, steps: int) -> torch.Tensor:
     if x.numel() == 0:
         return out
     batch = x.numel() // (rows * cols)
-    plan = get_plan(tuple((i * rows * cols, rows, cols) for i in range(batch)), x.device)
+    plan = get_plan((batch, rows, cols), lambda: [(i * rows * cols, rows, cols) for i in range(batch)], x.device)
     plan.launch(inp=x, steps=steps, out=out)
     return out
 
@@ -331,4 +338,8 @@ def muon_step(plan: NsPlan, w: torch.Tensor, buf: torch.Tensor, g: torch.Tensor,
         hipk.require(w16, torch.bfloat16, "muon_step: w16")
     if buf.numel() != n or g.numel() != n or (w16 is not None and w16.numel() != n) or hyper.numel() != 2:
         raise ValueError("muon_step: buffer sizes differ")
+    if any(t is not None and t.device != w.device for t in (buf, g, w16, hyper)):
+        raise ValueError("muon_step: buffers on different devices")
+    if not 1 <= steps <= MAX_STEPS:
+        raise ValueError("muon_step: steps must be from 1 to %d, got %r" % (MAX_STEPS, steps))
     plan.launch(inp=g, steps=steps, buf=buf, w=w, w16=w16, hyper=hyper, mu=float(mu), wd=float(wd), nesterov=nesterov)

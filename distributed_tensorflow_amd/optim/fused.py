@@ -250,7 +250,7 @@ class FusedMuon(_RegionOptimizer):
             if r.matrices:
                 self.buf[r.name] = torch.zeros_like(r.w)
                 if r.w.is_cuda:
-                    self._plans[r.name] = ns.NsPlan(r.matrices, r.w.device)
+                    self._plans[r.name] = ns.get_plan(tuple(map(tuple, r.matrices)), lambda: r.matrices, r.w.device)
             if r.vectors:
                 self.m[r.name] = torch.zeros_like(r.w)
                 self.v[r.name] = torch.zeros_like(r.w)

@@ -140,6 +140,8 @@ def train_input_fn(tfrecords_path, params, device, rank, world, channels=8):
 
 
 def _head_kwargs(model_name):
+    if FLAGS.head_norm not in ("none", "layer"):
+        raise ValueError("--head_norm must be none or layer, not %r" % FLAGS.head_norm)
     if FLAGS.head_norm == "none":
         return {}
     if model_name == "resnet50":
@@ -447,7 +449,9 @@ def main(unused_argv):
 
     print(os.environ.get("TF_CONFIG"))
     spec = parse_tf_config()
-    _optimizer_config()  # (a combination that cannot run ends every task at once, none waits for the others)
+    # (a combination that cannot run ends every task at once, none waits for the others)
+    _optimizer_config()
+    _head_kwargs(FLAGS.model)
     if spec.task_type == "ps":
         return run_ps(spec)
     if spec.task_type == "evaluator":

@@ -341,9 +341,17 @@ def test_muon_step_refusals():
     hyper = torch.zeros(2, device="cuda")
     good = dict(w=w, buf=w.clone(), g=w.clone(), w16=None, hyper=hyper, mu=0.9, wd=0.0, nesterov=True, steps=5)
     for name, t in [("w", w.bfloat16()), ("buf", w[:16]), ("g", w.half()), ("g", w[::2]), ("w16", w), ("hyper", hyper[:1]),
-                    ("w", w.cpu()), ("g", w.cpu())]:
+                    ("w", w.cpu()), ("g", w.cpu()), ("steps", 0), ("steps", ns.MAX_STEPS + 1)]:
         with pytest.raises(ValueError):
             ns.muon_step(plan, **{**good, name: t})
+
+
+@pytest.mark.parametrize("matrices", [[(0, 4, 8), (32, 1, 1)], [(1, 4, 8)], [(-1, 4, 8)]])
+def test_a_plan_that_does_not_fit_its_buffers_is_refused(matrices):
+    plan = ns.NsPlan(matrices, torch.device("cuda", 0))
+    w = torch.zeros(32, device="cuda")
+    with pytest.raises(ValueError, match="plan"):
+        ns.muon_step(plan, w, w.clone(), w.clone(), None, torch.zeros(2, device="cuda"), 0.9, 0.0, True, 5)
 
 
 def test_model_trains_with_muon_and_matches_the_cpu():

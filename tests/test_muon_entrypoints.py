@@ -59,3 +59,13 @@ def test_modes_that_cut_matrices_end_at_once(tmp_path):
                             "--checkpoint_dir=%s/ckpt/" % tmp_path, "--device=cpu"], cwd=DIST, env=env,
                            stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=120)
         assert r.returncode != 0 and "whole matrices" in r.stdout, r.stdout
+
+
+def test_an_unknown_head_norm_ends_every_task_at_once(tmp_path):
+    cluster = {"ps": ["localhost:%d" % _port()], "worker": ["localhost:%d" % _port()]}
+    for task in ("ps", "worker"):
+        env = dict(os.environ, TF_CONFIG=json.dumps({"cluster": cluster, "task": {"type": task, "index": 0}}))
+        r = subprocess.run([sys.executable, "train_dataset.py", "--synthetic", "--mode=async_ps", "--head_norm=batch",
+                            "--checkpoint_dir=%s/ckpt/" % tmp_path, "--device=cpu"], cwd=DIST, env=env,
+                           stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=120)
+        assert r.returncode != 0 and "head_norm" in r.stdout, r.stdout
