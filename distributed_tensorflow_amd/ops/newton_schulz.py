@@ -7,7 +7,6 @@ allocator, so calls on different streams, and captured graphs, never share one.
 from __future__ import annotations
 
 import ctypes as C
-import heapq
 import math
 from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
@@ -30,6 +29,7 @@ CHUNK = 8192              # elements per partial sum, at least
 # of them for 256 CUs.
 JOB_US = {128: 5.0, 64: 1.5}
 STEP_US = {128: 0.72, 64: 0.31}
+JOIN_US, JOIN_US_PER_BYTE = 4.0, 0.25e-6   # the launch that joins cut reductions (8 MB of slabs 6 us, 127 MB 36 us)
 CUS = 256
 SLOTS = 2 * CUS           # workgroups at a time
 MIN_STEPS = 8             # shortest piece of a cut reduction
@@ -95,32 +95,26 @@ def _up(v: int, edge: int) -> int:
 
 
 def _span(jobs: Sequence[Tuple[int, float]]) -> float:
-    """Time of a launch of (count, cost) jobs, longest first: an even share per CU (two workgroups share a CU's matrix
-    cores, so what counts is the work per CU), or what the CU with the most of the longest jobs takes."""
-    span = count = total = 0.0
+    """Time of a launch of (count, cost) jobs, longest first.  Two workgroups share a CU's matrix cores, so what counts is
+    the work per CU, or what the CU with the most of the longest jobs takes; and a long job that started first has had half
+    a CU for as long as there were others to start.  (ResNet-50's A stage in 35 cuttings, 55 .. 130 us: within 15 % of the
+    measured times; without the last term the best by estimate took 84 us where the best takes 67.)"""
+    span = count = total = longest = 0.0
     for n, cost in sorted(jobs, key=lambda j: -j[1]):
+        longest = longest or cost
         count += n
         total += n * cost
         span = max(span, math.ceil(count / CUS) * cost)
-    return max(span, total / CUS * 1.08)
-
-
-def _dealt(jobs: Sequence[Tuple[int, float]]) -> float:
-    """The same, job by job: longest first, each to the CU that is free first.  (ResNet-50's A stage in 22 cuttings: within
-    10 % of the measured times, 61 .. 125 us; the two bounds of ``_span`` alone miss what uneven jobs leave idle.)"""
-    free = [0.0] * CUS
-    for n, cost in sorted(jobs, key=lambda j: -j[1]):
-        for _ in range(n):
-            heapq.heapreplace(free, free[0] + cost)
-    return max(free)
+    share = total / CUS
+    return max(span, share * 1.08, longest + share / 2 if count > 0.9 * CUS else 0.0)
 
 
 def _choose(dims: Sequence[Tuple[int, int, int]], symmetric: bool) -> Tuple[int, int]:
     """(size of the shorter of tile rows / columns from which tiles are 128, longest piece of a reduction in k-steps) of a
     stage whose outputs are ``rows x cols`` sums over ``K`` for (rows, cols, K) in ``dims``."""
-    options = []
+    best: Optional[Tuple[float, int, int]] = None
     for large_from in (128, 256, 512, 1024, 1 << 30):
-        for piece in (1 << 30, 64, 48, 32, 24, 16, MIN_STEPS) if symmetric else (1 << 30,):
+        for piece in (1 << 30, 64, 48, 40, 32, 28, 24, 20, 16, 12, MIN_STEPS) if symmetric else (1 << 30,):
             jobs: Dict[float, int] = {}
             slabs = 0
             for rows, cols, K in dims:
@@ -131,13 +125,14 @@ def _choose(dims: Sequence[Tuple[int, int, int]], symmetric: bool) -> Tuple[int,
                 cost = _job_us(edge, -(-steps // cut))
                 jobs[cost] = jobs.get(cost, 0) + n * cut
                 slabs += n * cut * edge * edge * 4 if cut > 1 else 0
-            counts = [(n, cost) for cost, n in jobs.items()]
-            options.append((_span(counts), 4.0 + slabs * 2 / 3e6 if slabs else 0.0, large_from, piece, counts))
-    # the few that may be best, job by job
-    options.sort(key=lambda o: o[0] + o[1])
-    few = [o for o in options[:4] if sum(n for n, _ in o[4]) <= 4096] or options[:1]
-    best = min(few, key=lambda o: (_dealt(o[4]) if len(few) > 1 else o[0]) + o[1])
-    return best[2], best[3]
+            if symmetric and len(dims) == 1 and cut == 1 and _tail(n):   # (the tail's work is spread by _cut_tail)
+                jobs[cost] = n - _tail(n)
+                jobs[cost * _tail(n) / CUS] = CUS
+                slabs = SLOTS * edge * edge * 4
+            time = _span([(n, cost) for cost, n in jobs.items()]) + (JOIN_US + slabs * JOIN_US_PER_BYTE if slabs else 0.0)
+            if best is None or time < best[0]:
+                best = (time, large_from, piece)
+    return best[1], best[2]
 
 
 def _cut(jobs: np.ndarray, piece: int, slabs: int) -> Tuple[np.ndarray, np.ndarray, int]:
@@ -157,11 +152,16 @@ def _cut(jobs: np.ndarray, piece: int, slabs: int) -> Tuple[np.ndarray, np.ndarr
     return out, joins, slabs + len(out) * unit
 
 
+def _tail(n: int) -> int:
+    """How many of ``n`` equal jobs lie beyond whole rounds of workgroups and would run on a mostly idle card."""
+    tail = n % SLOTS
+    return tail if n >= SLOTS and tail <= SLOTS // 2 else 0
+
+
 def _cut_tail(jobs: np.ndarray, slabs: int) -> Tuple[np.ndarray, np.ndarray, int]:
-    """Equal jobs beyond whole rounds of workgroups would run on a mostly idle card: their reductions are cut so that all
-    of it takes part."""
-    tail = len(jobs) % SLOTS
-    if len(jobs) < SLOTS or not 0 < tail <= SLOTS // 2:
+    """The reductions of such jobs are cut so that the whole card takes part."""
+    tail = _tail(len(jobs))
+    if not tail:
         return jobs, jobs[:0], slabs
     steps = int(jobs[0, 5] - jobs[0, 4]) // 32
     piece = max(MIN_STEPS, -(-steps // max(2, SLOTS // tail)))
