@@ -24,6 +24,13 @@
 // tile row, tile column), longest first.  The operands live in a workspace whose planes are padded with zeros to whole
 // tiles, so the products need no bounds checks; a row holds its two planes in turns of 32 values, hi then lo, so that the
 // 32 k of a step are one 128-byte line per row (apart, each plane's 64 bytes fetched a line of which half was used).
+//
+// Measured: 4096 x 4096, an iteration A 199 us, B 202 us, X 375 us: 1.05 .. 1.1 PFLOP/s in the matrix cores, next to 1.45
+// of the fastest large fp16 product on this card, matrix cores busy two thirds of the time at a clock that the power limit
+// holds at 1.65 .. 1.8 GHz.  ResNet-50's 54 matrices, an iteration A 62 + 12, B 30, X 107 us: X's tiles have as few as two
+// k-steps, so that what they take is their first loads and the 128 KB of X that each reads and writes at its end; norm and first iterate 55 and
+// 64 us at 5 TB/s, the last X with the parameters 133.  Up to a few hundred rows an iteration is four launches of 4 .. 15 us,
+// a tile's own latency.
 #include "row_io.h"
 
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));

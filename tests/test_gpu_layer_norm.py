@@ -73,7 +73,9 @@ SIZES = [(1, 1), (2, 3), (1, 8), (5, 7), (9, 64), (4, 65), (33, 128), (1030, 72)
          (67, 2049), (31, 4100), (7, 8200), (5, 16390), (3, 33001), (2, 40000), (4099, 16), (301, 136), (77, 191), (70, 330), (19, 760), (11, 1500),
          # more rows than the one-launch form takes
          (1100, 136), (1030, 200), (1029, 520), (1040, 1001), (1027, 1500), (1030, 2049), (1030, 4100), (1026, 8200), (1025, 16390),
-         (1024, 2048), (1024, 2050)]
+         (1024, 2048), (1024, 2050),
+         # the longest rows of fp32 that the backward holds
+         (3, 16381), (600, 16384)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
