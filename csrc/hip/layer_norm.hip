@@ -21,10 +21,10 @@
 //
 // All arithmetic is fp32; outputs are rounded once.
 //
-// Measured (a copy of 1 GiB runs at 5.2 TB/s): 2^27 bf16 or 2^26 fp32 elements, forward 4.2 .. 5.7 TB/s and backward
-// 4.6 .. 5.6 for rows of 64 to 8192 elements (128 us and 176 us the slowest, 136 columns of bf16); 16384 columns of bf16 4.7
-// both ways.  The looping kernels, from 16385 columns of bf16 or 8193 of fp32 (forward 32769 and 16385): forward 3.5 .. 4.1
-// at 32768, backward 2.6, as it reads every row twice and both columns' sums once more.
+// Measured (a copy of 1 GiB runs at 5.2 TB/s): 2^27 bf16 or 2^26 fp32 elements in rows of 64 to 16384, forward
+// 4.2 .. 5.8 TB/s (128 us the slowest, 136 columns of bf16) and backward 4.0 .. 5.6 (203 us, 2100 columns of bf16).  The
+// looping kernels: forward 3.4 TB/s at 32768 columns of fp32, backward 2.5 at 32768 of either, as it reads every row
+// twice and the columns' sums read it once more.
 #include "row_io.h"
 
 // VEC values of a per-column fp32 vector (gamma / beta), `fill` where there is none; with TAIL those behind column C are 0
@@ -617,9 +617,13 @@ static int ln_fwd(const LnFwd& p, long long nvec, hipStream_t st) {
   if (nvec <= 128) return ln_fwd_launch<T, 64, 2>(p, st);
   if (nvec <= 192) return ln_fwd_launch<T, 64, 3>(p, st);
   if (nvec <= 256) return ln_fwd_launch<T, 64, 4>(p, st);
+  if (nvec <= 384) return ln_fwd_launch<T, 128, 3>(p, st);
   if (nvec <= 512) return ln_fwd_launch<T, 256, 2>(p, st);
+  if (nvec <= 768) return ln_fwd_launch<T, 256, 3>(p, st);
   if (nvec <= 1024) return ln_fwd_launch<T, 256, 4>(p, st);
-  if (nvec <= 2048) return ln_fwd_launch<T, 1024, 2>(p, st);
+  if (nvec <= 1536) return ln_fwd_launch<T, 512, 3>(p, st);
+  if (nvec <= 2048) return ln_fwd_launch<T, 512, 4>(p, st);
+  if (nvec <= 3 * 1024) return ln_fwd_launch<T, 1024, 3>(p, st);
   if (nvec <= 4096) return ln_fwd_launch<T, 1024, 4>(p, st);
   const long long grid = p.rows < LN_MAX_GRID ? p.rows : LN_MAX_GRID;
   hipLaunchKernelGGL((layer_norm_fwd_long_kernel<T>), dim3((unsigned)grid), dim3(1024), 0, st, p);
@@ -701,8 +705,11 @@ static int ln_bwd(const LnBwd& p, long long nvec, int parts, float* dgamma, floa
   if (nvec <= 128) return ln_bwd_launch<T, 64, 2>(p, parts, dgamma, dbeta, st);
   if (nvec <= 192) return ln_bwd_launch<T, 64, 3>(p, parts, dgamma, dbeta, st);
   if (nvec <= 256) return ln_bwd_launch<T, 64, 4>(p, parts, dgamma, dbeta, st);
+  if (nvec <= 384) return ln_bwd_launch<T, 128, 3>(p, parts, dgamma, dbeta, st);
   if (nvec <= 512) return ln_bwd_launch<T, 128, 4>(p, parts, dgamma, dbeta, st);
+  if (nvec <= 768) return ln_bwd_launch<T, 256, 3>(p, parts, dgamma, dbeta, st);
   if (nvec <= 1024) return ln_bwd_launch<T, 256, 4>(p, parts, dgamma, dbeta, st);
+  if (nvec <= 1536) return ln_bwd_launch<T, 512, 3>(p, parts, dgamma, dbeta, st);
   if (nvec <= 2048) return ln_bwd_launch<T, 512, 4>(p, parts, dgamma, dbeta, st);
   if constexpr (sizeof(T) == 4)
     if (nvec <= 4096) return ln_bwd_launch<T, 1024, 4>(p, parts, dgamma, dbeta, st);

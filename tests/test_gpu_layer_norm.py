@@ -75,7 +75,8 @@ SIZES = [(1, 1), (2, 3), (1, 8), (5, 7), (9, 64), (4, 65), (33, 128), (1030, 72)
          (1100, 136), (1030, 200), (1029, 520), (1040, 1001), (1027, 1500), (1030, 2049), (1030, 4100), (1026, 8200), (1025, 16390),
          (1024, 2048), (1024, 2050),
          # the longest rows of fp32 that the backward holds
-         (3, 16381), (600, 16384)]
+         (3, 16381), (600, 16384),
+         (6, 2900), (6, 3301), (5, 6201), (5, 12001), (5, 14001), (4, 24001), (1030, 2900), (1029, 6201), (1026, 12001)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
