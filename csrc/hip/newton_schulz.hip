@@ -25,12 +25,11 @@
 // tiles, so the products need no bounds checks; a row holds its two planes in turns of 32 values, hi then lo, so that the
 // 32 k of a step are one 128-byte line per row (apart, each plane's 64 bytes fetched a line of which half was used).
 //
-// Measured: 4096 x 4096, an iteration A 199 us, B 202 us, X 375 us: 1.05 .. 1.1 PFLOP/s in the matrix cores, next to 1.45
-// of the fastest large fp16 product on this card, matrix cores busy two thirds of the time at a clock that the power limit
-// holds at 1.65 .. 1.8 GHz.  ResNet-50's 54 matrices, an iteration A 62 + 12, B 30, X 107 us: X's tiles have as few as two
-// k-steps, so that what they take is their first loads and the 128 KB of X that each reads and writes at its end; norm and first iterate 55 and
-// 64 us at 5 TB/s, the last X with the parameters 133.  Up to a few hundred rows an iteration is four launches of 4 .. 15 us,
-// a tile's own latency.
+// Measured: 4096 x 4096, an iteration A 188 us, B 191 us, X 355 us: 1.1 .. 1.2 PFLOP/s in the matrix cores, next to 1.45
+// of the fastest large fp16 product on this card.  ResNet-50's 54 matrices, an iteration A 58 + 12, B 30, X 106 us: X's
+// tiles have as few as two k-steps, so that what they take is their first loads and the 128 KB of X that each reads and
+// writes at its end; norm and first iterate 55 and 64 us at 5 TB/s, the last X with the parameters 134.  Up to a few hundred
+// rows an iteration is four launches of 4 .. 15 us, 5 of them a tile's first loads and its end.
 #include "row_io.h"
 
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
@@ -243,6 +242,19 @@ struct NsOperand {
   int i0;
 };
 
+// 16 bytes a lane from `base` (the same for the wave) + `off` into LDS at `lds` + AT, lane after lane.  No other code of a
+// kernel keeps a value in m0.
+template <int AT>
+__device__ __forceinline__ void ns_to_stage(const f16* base, unsigned off, unsigned lds) {
+  asm volatile(
+      "s_add_u32 m0, %2, %3\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %0, %1"
+      :
+      : "v"(off), "s"(base), "s"(lds), "n"(AT)
+      : "memory", "scc", "m0");
+}
+
 // T x T tile of sum_k P(i, k) Q(j, k), k0 <= k < k1, on 2 x 2 waves.  The accumulator of a wave holds the TRANSPOSED tile
 // (Q is the matrix instruction's first operand): lane l, element e of acc[u][v] is column
 // j = v * 32 + (e & 3) + 8 (e >> 2) + 4 (l >> 5) of row i = u * 32 + (l & 31), so four consecutive elements are four
@@ -251,6 +263,10 @@ struct NsOperand {
 // k advances by 32; each of the four waves brings half of an operand of the next k-tiles (P, P, Q, Q) into LDS by
 // LDS-DMA, NST - 1 k-tiles ahead, with counted waits and raw barriers; the fragments of the next 16 k are read while the
 // matrix instructions of the present ones run.
+//
+// What bounds it is LDS: a k-tile of 128 x 128 is 32 KB written and 64 KB read, 768 cycles at 128 bytes a cycle, next to
+// 768 cycles of matrix instructions on each of the four SIMDs; one of 64 x 64 is 48 KB, 384 cycles, next to 192 (and takes
+// 475 where a workgroup has its CU to itself).
 template <int T, bool PK, bool QK>
 __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& Q, int k0, int k1, char* smem,
                                            f32x16 (&acc)[T / 64][T / 64]) {
@@ -263,69 +279,92 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wid >> 1, wc = wid & 1;
 
-  // staging: this wave's half of an operand
+  // staging: this wave's half of an operand.  What stands beside the matrix instructions is kept short: the offsets of the
+  // lanes in registers, the k-tiles' start in scalar ones, places in LDS as constants of a loop over the slots (with all of
+  // it computed anew for every k-tile: 4096 x 4096 A 199, B 202, X 375 us instead of 188, 191 and 355).
   const bool kmajor = wid < 2 ? PK : QK;
-  const f16* base = wid < 2 ? P.base : Q.base;
   const int ld = wid < 2 ? P.ld : Q.ld, i0 = wid < 2 ? P.i0 : Q.i0;
-  const f16* src[2];  // of the even and of the odd instructions
-  size_t pair, step;  // elements between the rows of two instructions, between two k-tiles
+  const f16* src = wid < 2 ? P.base : Q.base;
+  unsigned off[LPS];                          // bytes: at most 128 rows of 2^20 columns
+  size_t step;                                // elements between two k-tiles
   if (kmajor) {
     constexpr int RPI = 256 / T;              // k rows per instruction: 2 or 4; this wave brings 16
 #pragma unroll
-    for (int o = 0; o < 2; ++o) {
-      const int r = (wid & 1) * 16 + o * RPI + lane / (64 / RPI), slot = lane % (64 / RPI);
-      src[o] = base + (size_t)(k0 + r) * 2 * ld + 2 * i0 + ((slot ^ ns_swz_tr(r)) << 3);
+    for (int i = 0; i < LPS; ++i) {
+      const int r = (wid & 1) * 16 + i * RPI + lane / (64 / RPI), slot = lane % (64 / RPI);
+      off[i] = (unsigned)r * 4 * ld + ((slot ^ ns_swz_tr(r)) << 4);
     }
-    pair = (size_t)4 * RPI * ld;
+    src += (size_t)k0 * 2 * ld + 2 * i0;
     step = (size_t)NS_BK * 2 * ld;
   } else {
 #pragma unroll
-    for (int o = 0; o < 2; ++o) {             // 8 rows per instruction
-      const int r = (wid & 1) * (T / 2) + o * 8 + (lane >> 3), slot = lane & 7;
-      src[o] = base + (size_t)(i0 + r) * 2 * ld + 2 * k0 + ((slot ^ ns_swz(r)) << 3);
+    for (int i = 0; i < LPS; ++i) {           // 8 rows per instruction
+      const int r = (wid & 1) * (T / 2) + i * 8 + (lane >> 3), slot = lane & 7;
+      off[i] = (unsigned)r * 4 * ld + ((slot ^ ns_swz(r)) << 4);
     }
-    pair = (size_t)32 * ld;
+    src += (size_t)i0 * 2 * ld + 2 * k0;
     step = 2 * NS_BK;
   }
-  // (the swizzles repeat every 16 rows, or 4: every second instruction finds the same slots)
-  auto stage_one = [&](int buf, int i) {
-    glds16_untracked(src[i & 1] + (i >> 1) * pair, smem + buf * STAGE + wid * (OPER / 2) + i * 1024);
-    if (i == LPS - 2) src[0] += step;
-    if (i == LPS - 1) src[1] += step;
-  };
-  auto stage = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < LPS; ++i) stage_one(buf, i);
+  // (a scalar register that the vector unit wrote can be read as an address five instructions later; where that is left to
+  // the compiler it counts them, behind inline assembly it does not look)
+  asm volatile("s_nop 4");
+  const unsigned lds = (unsigned)(uintptr_t)(LDS_AS char*)smem;
+  const unsigned lds_wave = lds + wid * (OPER / 2);
+  // (`i` and the slot are constants once the loops around are unrolled)
+  auto stage_one = [&](int slot, int i) {
+    const unsigned at = lds_wave + slot * STAGE;
+    if (i == 0) ns_to_stage<0>(src, off[0], at);
+    if (i == 1) ns_to_stage<1024>(src, off[1], at);
+    if (i == 2) ns_to_stage<2048>(src, off[2], at);
+    if (i == 3) ns_to_stage<3072>(src, off[3], at);
+    if constexpr (LPS == 8) {
+      if (i == 4) ns_to_stage<4096>(src, off[4], at);
+      if (i == 5) ns_to_stage<5120>(src, off[5], at);
+      if (i == 6) ns_to_stage<6144>(src, off[6], at);
+      if (i == 7) ns_to_stage<7168>(src, off[7], at);
+    }
+    if (i == LPS - 1) src += step;
   };
 
-  // fragments
-  const int tr_q = (lane & 15) >> 2;
-  const int tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-  const int tr_k = 8 * (lane >> 5) + tr_q;
-  auto frag = [&](const char* oper, bool km, int row0, int ks, int lo) -> f16x8 {
+  // fragments: a lane's places in the first slot, for the two planes and, where the swizzle mixes them with the place,
+  // the halves of k (k contiguous) or the blocks of 32 rows (k-major); everything else is a constant to add
+  auto places = [&](bool km, int row0, unsigned oper, unsigned (&at)[2][2]) {
+#pragma unroll
+    for (int lo = 0; lo < 2; ++lo)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (km) {
+          const int col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3), krow = 8 * (lane >> 5) + ((lane & 15) >> 2);
+          const int chunk = ((row0 >> 5) + x) * 8 + lo * 4 + (col >> 3);
+          at[lo][x] = lds + oper + krow * (T * 4) + ((chunk ^ ns_swz_tr(krow)) << 4) + (col & 7) * 2;
+        } else {
+          const int row = row0 + (lane & 31);
+          at[lo][x] = lds + oper + row * 128 + (((lo * 4 + x * 2 + (lane >> 5)) ^ ns_swz(row)) << 4);
+        }
+      }
+  };
+  unsigned p_at[2][2], q_at[2][2];
+  places(PK, wr * (T / 2), 0, p_at);
+  places(QK, wc * (T / 2), OPER, q_at);
+  auto frag = [&](bool km, const unsigned (&at)[2][2], int slot, int u, int ks, int lo) -> f16x8 {
     if (km) {
       union { s16x4 h[2]; f16x8 v; } r;
-      const int chunk = (row0 >> 5) * 8 + lo * 4 + (tr_col >> 3);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int krow = ks * 16 + tr_k + 4 * q;
-        const char* at = oper + krow * (T * 4) + ((chunk ^ ns_swz_tr(krow)) << 4) + (tr_col & 7) * 2;
-        r.h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)at);
-      }
+      for (int q = 0; q < 2; ++q)
+        r.h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (LDS_AS s16x4*)(uintptr_t)(at[lo][u] + slot * STAGE + (ks * 16 + 4 * q) * (T * 4)));
       return r.v;
     }
-    const int row = row0 + (lane & 31);
-    return *(const f16x8*)(oper + row * 128 + (((lo * 4 + ks * 2 + (lane >> 5)) ^ ns_swz(row)) << 4));
+    return *(const LDS_AS f16x8*)(uintptr_t)(at[lo][ks] + slot * STAGE + u * 4096);
   };
   f16x8 ph[2][MT], pl[2][MT], qh[2][MT], ql[2][MT];
   constexpr int FRAGS = 4 * MT;               // of a step of 16 k: Q hi, P hi, Q lo, P lo
-  auto load_frag = [&](int buf, int ks, int to, int i) {
-    const char* at = smem + buf * STAGE;
+  auto load_frag = [&](int slot, int ks, int to, int i) {
     const int u = i % MT;
-    if (i / MT == 0) qh[to][u] = frag(at + OPER, QK, wc * (T / 2) + u * 32, ks, 0);
-    if (i / MT == 1) ph[to][u] = frag(at, PK, wr * (T / 2) + u * 32, ks, 0);
-    if (i / MT == 2) ql[to][u] = frag(at + OPER, QK, wc * (T / 2) + u * 32, ks, 1);
-    if (i / MT == 3) pl[to][u] = frag(at, PK, wr * (T / 2) + u * 32, ks, 1);
+    if (i / MT == 0) qh[to][u] = frag(QK, q_at, slot, u, ks, 0);
+    if (i / MT == 1) ph[to][u] = frag(PK, p_at, slot, u, ks, 0);
+    if (i / MT == 2) ql[to][u] = frag(QK, q_at, slot, u, ks, 1);
+    if (i / MT == 3) pl[to][u] = frag(PK, p_at, slot, u, ks, 1);
   };
   // the matrix instructions of a step of 16 k; `between` issues other work behind each, which runs in its shadow
   auto multiply = [&](int from, auto between) {
@@ -349,6 +388,10 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
       for (int e = 0; e < 16; ++e) acc[u][v][e] = 0.f;
 
   const int nk = (k1 - k0) / NS_BK;
+  auto stage = [&](int slot) {
+#pragma unroll
+    for (int i = 0; i < LPS; ++i) stage_one(slot, i);
+  };
 #pragma unroll
   for (int s = 0; s < NST - 1; ++s)
     if (s < nk) stage(s);
@@ -364,39 +407,44 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
   if (NST - 1 < nk) stage(NST - 1);
 #pragma unroll
   for (int i = 0; i < FRAGS; ++i) load_frag(0, 0, 0, i);
-  int cur = 0;
   // Issued in a block, the eight LDS-DMA and eight LDS reads of a step would hold the wave for as long as its matrix
   // instructions take; one behind each of these they cost next to nothing.
-  // (The last k-tile stands by itself: with one loop for all, the wait counts in front of the second group would have to
-  // hold for the pass without new reads as well, and wait for the new reads in all others.)
   constexpr int N = 3 * MT * MT;
   constexpr int RPM = (FRAGS + N - 1) / N;    // reads, and LDS-DMA, behind one matrix instruction
   constexpr int SPM = (LPS + N - 1) / N;
-  for (int kt = 0; kt + 1 < nk; ++kt) {
-    const int nxt = cur == NST - 1 ? 0 : cur + 1;
+  auto second_half = [&](int slot) {
     multiply(0, [&](int n) {
 #pragma unroll
       for (int i = n * RPM; i < n * RPM + RPM; ++i)
-        if (i < FRAGS) load_frag(cur, 1, 1, i);
+        if (i < FRAGS) load_frag(slot, 1, 1, i);
     });
-    arrive(kt + 1);  // ... and k-tile kt has been read by every wave: its slot takes k-tile kt + NST
-    const bool more = kt + NST < nk;
-    multiply(1, [&](int n) {
+  };
+  // (The last k-tile stands by itself: with one loop for all, the wait counts in front of the second group would have to
+  // hold for the pass without new reads as well, and wait for the new reads in all others.)
+  int last = -1;  // its slot
+  for (int kt = 0; last < 0; kt += NST) {
 #pragma unroll
-      for (int i = n * RPM; i < n * RPM + RPM; ++i)
-        if (i < FRAGS) load_frag(nxt, 0, 0, i);
-      if (more)
+    for (int slot = 0; slot < NST; ++slot) {
+      const int nxt = (slot + 1) % NST;
+      if (kt + slot + 1 == nk) {
+        last = slot;
+        break;
+      }
+      second_half(slot);
+      arrive(kt + slot + 1);  // ... and this k-tile has been read by every wave: its slot takes the one NST further on
+      const bool more = kt + slot + NST < nk;
+      multiply(1, [&](int n) {
 #pragma unroll
-        for (int i = n * SPM; i < n * SPM + SPM; ++i)
-          if (i < LPS) stage_one(cur, i);
-    });
-    cur = nxt;
+        for (int i = n * RPM; i < n * RPM + RPM; ++i)
+          if (i < FRAGS) load_frag(nxt, 0, 0, i);
+        if (more)
+#pragma unroll
+          for (int i = n * SPM; i < n * SPM + SPM; ++i)
+            if (i < LPS) stage_one(slot, i);
+      });
+    }
   }
-  multiply(0, [&](int n) {
-#pragma unroll
-    for (int i = n * RPM; i < n * RPM + RPM; ++i)
-      if (i < FRAGS) load_frag(cur, 1, 1, i);
-  });
+  second_half(last);
   multiply(1, [](int) {});
 }
 

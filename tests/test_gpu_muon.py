@@ -147,6 +147,12 @@ def test_large_matrix():
     assert off <= (8 + math.sqrt(3 * 4096 / 16)) * base + 2.0 ** -23 * want.norm().item()
 
 
+@pytest.mark.parametrize("rows,cols", [(100, 1 << 20), (1 << 20, 70)])
+def test_longest_side(rows, cols):
+    g = _matrix(rows, cols, torch.float32, 12)
+    _check(F.orthogonalize(g, steps=1), g, 1)
+
+
 def test_rank_one():
     u, v = _matrix(200, 1, torch.float32, 11), _matrix(1, 333, torch.float32, 12)
     g = (u @ v) * 1e6
