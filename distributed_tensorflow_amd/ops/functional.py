@@ -1043,7 +1043,7 @@ class _LayerNormFn(Function):
     def backward(ctx, dy):
         x, gamma, stats = ctx.saved_tensors
         want_dx, want_dg, want_db = ctx.needs_input_grad[:3]
-        dx, dg, db = K.layer_norm_bwd(dy, x, gamma, stats, want_dx, want_dg, want_db)
+        dx, dg, db = K.layer_norm_bwd_checked(dy, x, gamma, stats, want_dx, want_dg, want_db)
         pg, pb = ctx.params
         if hasattr(pg, "main_grad"):
             dg = _deliver_small(pg, dg)

@@ -9,6 +9,7 @@ from __future__ import annotations
 import os
 
 import ctypes as C
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -595,6 +596,11 @@ def layer_norm_fwd(x: torch.Tensor, gamma: Optional[torch.Tensor], beta: Optiona
     return y, stats
 
 
+@functools.lru_cache(maxsize=1024)
+def _ln_parts(rows: int, cols: int, dtype: int) -> int:
+    return hipk.lib().dtfa_layer_norm_bwd_parts(rows, cols, dtype)
+
+
 def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, gamma: Optional[torch.Tensor], stats: torch.Tensor,
                    want_dx: bool = True, want_dgamma: bool = True, want_dbeta: bool = True):
     """Gradients ``(dx, dgamma, dbeta)`` of :func:`layer_norm_fwd`, None where not wanted.  ``dgamma`` / ``dbeta`` (fp32)
@@ -603,24 +609,35 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, gamma: Optional[torch.Tens
     if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
         raise ValueError("layer_norm backward: dy %s %s does not match x %s %s"
                          % (tuple(dy.shape), dy.dtype, tuple(x.shape), x.dtype))
-    cols = x.shape[-1]
-    rows = x.numel() // cols
+    rows = x.numel() // x.shape[-1]
     hipk.require(stats, F32, "layer_norm: stats")
     if stats.shape != (2, rows) or stats.device != x.device:
         raise ValueError("layer_norm backward: stats must be two values for each of %d rows, got shape %s"
                          % (rows, tuple(stats.shape)))
+    return layer_norm_bwd_checked(dy, x, gamma, stats, want_dx, want_dgamma, want_dbeta)
+
+
+def layer_norm_bwd_checked(dy, x, gamma, stats, want_dx, want_dgamma, want_dbeta):
+    """:func:`layer_norm_bwd` of what a forward pass checked and autograd hands back (small calls are bound by the host)."""
+    cols = x.shape[-1]
+    rows = x.numel() // cols
     with hipk.device_of(x):
         dx = _ln_like(x) if want_dx else None
-        fresh = torch.empty if rows else torch.zeros
-        dgamma = fresh(cols, dtype=F32, device=x.device) if want_dgamma else None
-        dbeta = fresh(cols, dtype=F32, device=x.device) if want_dbeta else None
+        if rows and gamma is not None:   # (empty_like: half the host time of empty with everything spelt out)
+            dgamma = torch.empty_like(gamma) if want_dgamma else None
+            dbeta = torch.empty_like(gamma) if want_dbeta else None
+        else:
+            fresh = torch.empty if rows else torch.zeros
+            dgamma = fresh(cols, dtype=F32, device=x.device) if want_dgamma else None
+            dbeta = fresh(cols, dtype=F32, device=x.device) if want_dbeta else None
         if rows:
             L, dt = hipk.lib(), _LN_DTYPES[x.dtype]
             (xr, ldx), (gr, ldg) = _ln_rows(x), _ln_rows(dy)
-            parts = L.dtfa_layer_norm_bwd_parts(rows, cols, dt) if want_dgamma or want_dbeta else 0
+            parts = _ln_parts(rows, cols, dt) if want_dgamma or want_dbeta else 0
             part = torch.empty(parts * 2 * cols, dtype=F32, device=x.device) if parts else None
             hipk.check(L.dtfa_layer_norm_bwd(xr.data_ptr(), ldx, gr.data_ptr(), ldg, hipk.ptr(gamma), stats.data_ptr(),
-                                             hipk.ptr(dx), hipk.ptr(part), hipk.ptr(dgamma), hipk.ptr(dbeta), rows, cols, dt, hipk.stream()), "layer_norm_bwd")
+                                             hipk.ptr(dx), hipk.ptr(part), hipk.ptr(dgamma), hipk.ptr(dbeta), rows, cols,
+                                             dt, hipk.stream()), "layer_norm_bwd")
     return dx, dgamma, dbeta
 
 
