@@ -265,14 +265,15 @@ __device__ __forceinline__ void ns_to_stage(const f16* base, unsigned off, unsig
 // matrix instructions of the present ones run.
 //
 // What bounds it is LDS: a k-tile of 128 x 128 is 32 KB written and 64 KB read, 768 cycles at 128 bytes a cycle, next to
-// 768 cycles of matrix instructions on each of the four SIMDs; one of 64 x 64 is 48 KB, 384 cycles, next to 192 (and takes
-// 475 where a workgroup has its CU to itself).
-template <int T, bool PK, bool QK>
+// 768 cycles of matrix instructions on each of the four SIMDs; one of 64 x 64 is 48 KB, 384 cycles, next to 192.  NST is 2
+// for 128 x 128.  64 x 64 tiles have three slots, so that three workgroups fit a CU, but A and B four where they are at most
+// two to a CU (36 tiles over 8192 values: 59 -> 46 us, with six no less; 872 tiles over up to 1024: 29.9 us with three slots,
+// 32.4 with four; 531 of X: 12.3 and 13.3).
+template <int T, int NST, bool PK, bool QK>
 __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& Q, int k0, int k1, char* smem,
                                            f32x16 (&acc)[T / 64][T / 64]) {
   constexpr int OPER = T * NS_BK * 4;         // bytes of an operand's k-tile, both planes
   constexpr int STAGE = 2 * OPER;
-  constexpr int NST = T == 128 ? 2 : 3;
   constexpr int LPS = OPER / 2048;            // LDS-DMA instructions per wave and k-tile
   constexpr int MT = T / 64;
   const int lane = threadIdx.x & 63;
@@ -450,10 +451,10 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
 
 // fp32 tile in LDS: 16-byte writes of 8 rows at a time hit every bank once at this pitch
 #define NS_PITCH(T) ((T) + 4)
-// LDS of a launch with large tiles (two workgroups to a CU), and of one without (three)
+// LDS of a launch with large tiles or four slots (two workgroups to a CU), and of others (three)
 #define NS_LDS_LARGE (128 * NS_PITCH(128) * 4)
 #define NS_LDS_SMALL (3 * 4 * 64 * NS_BK * 2)
-static_assert(NS_LDS_LARGE >= 2 * 4 * 128 * NS_BK * 2 && NS_LDS_LARGE >= NS_LDS_SMALL, "stages fit");
+static_assert(NS_LDS_LARGE >= 2 * 4 * 128 * NS_BK * 2 && NS_LDS_LARGE >= 4 * 4 * 64 * NS_BK * 2, "stages fit");
 static_assert(NS_LDS_SMALL >= 64 * NS_PITCH(64) * 4, "the fp32 tile fits");
 
 // accumulators -> the tile [i][j] in LDS
@@ -514,18 +515,18 @@ __device__ __forceinline__ void ns_symmetric_out(const NsArgs& p, const NsMat& m
 }
 
 // Tile of A = X X^T (or X^T X) or, with POLY, of A A; with a slab, only the sums over the job's share of k.
-template <int T, bool POLY>
+template <int T, int NST, bool POLY>
 __device__ __forceinline__ void ns_symmetric(const NsArgs& p, const NsMat& m, const NsJob& job, int k, int lift, char* smem) {
   f32x16 acc[T / 64][T / 64];
   const f16* x = p.ws + m.x + (k & 1 ? (size_t)2 * m.rp * m.cp : 0);
   const f16* a = p.ws + m.a;
   const int i0 = job.ti * T, j0 = job.tj * T;
   if (POLY)
-    ns_product<T, false, false>({a, m.mp, i0}, {a, m.mp, j0}, job.k0, job.k1, smem, acc);
+    ns_product<T, NST, false, false>({a, m.mp, i0}, {a, m.mp, j0}, job.k0, job.k1, smem, acc);
   else if (m.tall)
-    ns_product<T, true, true>({x, m.cp, i0}, {x, m.cp, j0}, job.k0, job.k1, smem, acc);
+    ns_product<T, NST, true, true>({x, m.cp, i0}, {x, m.cp, j0}, job.k0, job.k1, smem, acc);
   else
-    ns_product<T, false, false>({x, m.cp, i0}, {x, m.cp, j0}, job.k0, job.k1, smem, acc);
+    ns_product<T, NST, false, false>({x, m.cp, i0}, {x, m.cp, j0}, job.k0, job.k1, smem, acc);
   float* tile = (float*)smem;
   ns_to_lds<T>(acc, tile);
   if (job.slab >= 0) {
@@ -588,6 +589,7 @@ __device__ __forceinline__ void ns_result(const NsArgs& p, const NsMat& m, int r
 template <int T, int WHAT, typename O>
 __device__ __forceinline__ void ns_advance(const NsArgs& p, const NsMat& m, const NsJob& job, int k, int lift, int lift_next,
                                            char* smem) {
+  constexpr int NST = T == 128 ? 2 : 3;
   f32x16 acc[T / 64][T / 64];
   const size_t xs = (size_t)2 * m.rp * m.cp;
   const f16* x = p.ws + m.x + (k & 1 ? xs : 0);
@@ -595,9 +597,9 @@ __device__ __forceinline__ void ns_advance(const NsArgs& p, const NsMat& m, cons
   const f16* b = p.ws + m.a + (size_t)2 * m.mp * m.mp;
   const int i0 = job.ti * T, j0 = job.tj * T;
   if (m.tall)
-    ns_product<T, false, false>({x, m.cp, i0}, {b, m.mp, j0}, job.k0, job.k1, smem, acc);
+    ns_product<T, NST, false, false>({x, m.cp, i0}, {b, m.mp, j0}, job.k0, job.k1, smem, acc);
   else
-    ns_product<T, false, true>({b, m.mp, i0}, {x, m.cp, j0}, job.k0, job.k1, smem, acc);
+    ns_product<T, NST, false, true>({b, m.mp, i0}, {x, m.cp, j0}, job.k0, job.k1, smem, acc);
   float* tile = (float*)smem;
   ns_to_lds<T>(acc, tile);
   const float lr = WHAT == NS_APPLY ? p.hyper[0] : 0.f;
@@ -625,7 +627,7 @@ __device__ __forceinline__ void ns_advance(const NsArgs& p, const NsMat& m, cons
   }
 }
 
-template <bool POLY>
+template <bool POLY, int SLOTS>
 __global__ __launch_bounds__(256, 2) void ns_symmetric_kernel(NsArgs p, int k) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const NsJob job = (POLY ? p.poly : p.gram)[blockIdx.x];
@@ -633,9 +635,9 @@ __global__ __launch_bounds__(256, 2) void ns_symmetric_kernel(NsArgs p, int k) {
   const NsMat m = p.mats[job.mat];
   const int lift = POLY ? ns_lift(p, job.mat, k) : 0;
   if (job.edge == 128)
-    ns_symmetric<128, POLY>(p, m, job, k, lift, smem);
+    ns_symmetric<128, 2, POLY>(p, m, job, k, lift, smem);
   else
-    ns_symmetric<64, POLY>(p, m, job, k, lift, smem);
+    ns_symmetric<64, SLOTS, POLY>(p, m, job, k, lift, smem);
 }
 
 template <bool POLY>
@@ -929,6 +931,12 @@ static int ns_tiles(int blocks, bool large, const NsArgs& a, int k, hipStream_t 
 }
 
 template <bool POLY>
+static int ns_symmetric_tiles(int blocks, bool large, const NsArgs& a, int k, hipStream_t st) {
+  if (blocks <= 512) return ns_tiles<ns_symmetric_kernel<POLY, 4>>(blocks, true, a, k, st);
+  return ns_tiles<ns_symmetric_kernel<POLY, 3>>(blocks, large, a, k, st);
+}
+
+template <bool POLY>
 static int ns_join(int tiles, const NsArgs& a, int k, hipStream_t st) {
   hipLaunchKernelGGL((ns_join_kernel<POLY>), dim3(tiles, 128 / NS_JOIN_ROWS), dim3(256), 0, st, a, k);
   return (int)hipGetLastError();
@@ -969,9 +977,9 @@ extern "C" int dtfa_newton_schulz(const NsArgs* args, hipStream_t st) {
          : ns_first<float, false>(a, st);
   for (int k = 0; k < a.steps && rc == 0; ++k) {
     if (a.nsmall == 0) {
-      rc = ns_tiles<ns_symmetric_kernel<false>>(a.ngram, (a.large & 1) != 0, a, k, st);
+      rc = ns_symmetric_tiles<false>(a.ngram, (a.large & 1) != 0, a, k, st);
       if (rc == 0 && a.ngram_joins > 0) rc = ns_join<false>(a.ngram_joins, a, k, st);
-      if (rc == 0) rc = ns_tiles<ns_symmetric_kernel<true>>(a.npoly, (a.large & 2) != 0, a, k, st);
+      if (rc == 0) rc = ns_symmetric_tiles<true>(a.npoly, (a.large & 2) != 0, a, k, st);
       if (rc == 0 && a.npoly_joins > 0) rc = ns_join<true>(a.npoly_joins, a, k, st);
       if (rc != 0) break;
     }
