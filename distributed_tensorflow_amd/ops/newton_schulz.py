@@ -36,7 +36,7 @@ MIN_STEPS = 8             # shortest piece of a cut reduction
 
 # Shorter sides of at most 64 take one launch an iteration, in which every workgroup adds up the partial products of all
 # slices of its matrix (about 0.25 us each) and advances the 64 x 64 blocks of its own (about 2.5 us each): the time is
-# least at sqrt(10 * blocks) slices.  64 x 576 fp32: 46 us against 80 in separate stages, 64 x 4608: 81 against 108.
+# least at sqrt(10 * blocks) slices.  64 x 576 bf16: 46 us against 80 in separate stages, 64 x 4608: 81 against 108.
 SMALL_BLOCKS_PER_SLICE2 = 10.0
 SMALL_MAX_LONG = 8192
 
