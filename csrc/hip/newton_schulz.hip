@@ -25,10 +25,10 @@
 // tiles, so the products need no bounds checks; a row holds its two planes in turns of 32 values, hi then lo, so that the
 // 32 k of a step are one 128-byte line per row (apart, each plane's 64 bytes fetched a line of which half was used).
 //
-// Measured: 4096 x 4096, an iteration A 188 us, B 191 us, X 355 us: 1.1 .. 1.2 PFLOP/s in the matrix cores, next to 1.45
-// of the fastest large fp16 product on this card.  ResNet-50's 54 matrices, an iteration A 58 + 12, B 30, X 106 us: X's
+// Measured: 4096 x 4096, an iteration A 187 us, B 189 us, X 353 us: 1.1 .. 1.2 PFLOP/s in the matrix cores, next to 1.45
+// of the fastest large fp16 product on this card.  ResNet-50's 54 matrices, an iteration A 57 + 12, B 29, X 105 us: X's
 // tiles have as few as two k-steps, so that what they take is their first loads and the 128 KB of X that each reads and
-// writes at its end; norm and first iterate 55 and 64 us at 5 TB/s, the last X with the parameters 134.  Up to a few hundred
+// writes at its end; norm and first iterate 56 and 65 us at 5 TB/s, the last X with the parameters 132.  Up to a few hundred
 // rows an iteration is four launches of 4 .. 15 us, 5 of them a tile's first loads and its end.
 #include "row_io.h"
 
@@ -282,7 +282,7 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
 
   // staging: this wave's half of an operand.  What stands beside the matrix instructions is kept short: the offsets of the
   // lanes in registers, the k-tiles' start in scalar ones, places in LDS as constants of a loop over the slots (with all of
-  // it computed anew for every k-tile: 4096 x 4096 A 199, B 202, X 375 us instead of 188, 191 and 355).
+  // it computed anew for every k-tile: 4096 x 4096 A 199, B 202, X 375 us instead of 187, 189 and 353).
   const bool kmajor = wid < 2 ? PK : QK;
   const int ld = wid < 2 ? P.ld : Q.ld, i0 = wid < 2 ? P.i0 : Q.i0;
   const f16* src = wid < 2 ? P.base : Q.base;

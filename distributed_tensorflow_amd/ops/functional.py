@@ -1056,7 +1056,8 @@ def layer_norm(x, gamma=None, beta=None, eps: float = 1e-5):
     """Normalise every vector along the last axis of ``x`` to mean 0 and variance 1 (biased, ``eps`` added to it), then
     scale by ``gamma`` and shift by ``beta`` (vectors, either may be None).  On the GPU ``x`` is bf16, fp16 or fp32 --
     contiguous or a channel slice of a wider tensor; other layouts are copied first --, ``gamma`` / ``beta`` are fp32, and
-    the result is contiguous in ``x``'s dtype.  Differentiable once in all three."""
+    the result is contiguous in ``x``'s dtype.  Differentiable once in all three.  (As with every operator, a backward pass
+    over leaves can be captured into a graph only while no eager graph over the same leaves is alive.)"""
     if not _use_hip(x):
         if x.dim() < 1 or x.shape[-1] < 1:
             raise ValueError("layer_norm: the last axis must not be empty, got shape %s" % (tuple(x.shape),))
