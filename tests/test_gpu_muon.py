@@ -126,6 +126,19 @@ def test_any_cut_of_the_work(monkeypatch, rows, cols, large_from, piece):
         _check(o, m)
 
 
+@pytest.mark.parametrize("rows,cols", [(300, 340), (340, 300)])
+def test_more_small_tiles_than_two_to_a_cu(monkeypatch, rows, cols):
+    monkeypatch.setattr(ns, "_choose", lambda dims, symmetric: (1 << 30, 1 << 30))
+    n = 40
+    g = torch.stack([_matrix(rows, cols, torch.float32, 90 + s) for s in range(n)])
+    plan = ns.NsPlan([(s * rows * cols, rows, cols) for s in range(n)], g.device)
+    assert plan.counts[4] > 2 * ns.CUS and plan.counts[6] > 2 * ns.CUS   # tiles of A, of B
+    out = torch.empty_like(g)
+    plan.launch(inp=g, steps=5, out=out)
+    for o, m in zip(out[::13], g[::13]):
+        _check(o, m)
+
+
 def test_leftover_tiles(monkeypatch):
     # a whole round of workgroups and a few tiles more, whose reductions are cut
     monkeypatch.setattr(ns, "_choose", lambda dims, symmetric: (1 << 30, 1 << 30))
