@@ -315,14 +315,14 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
   auto stage_one = [&](int slot, int i) {
     const unsigned at = lds_wave + slot * STAGE;
     if (i == 0) ns_to_stage<0>(src, off[0], at);
-    if (i == 1) ns_to_stage<1024>(src, off[1], at);
-    if (i == 2) ns_to_stage<2048>(src, off[2], at);
-    if (i == 3) ns_to_stage<3072>(src, off[3], at);
+    if (i == 1) ns_to_stage<1 * 1024>(src, off[1], at);
+    if (i == 2) ns_to_stage<2 * 1024>(src, off[2], at);
+    if (i == 3) ns_to_stage<3 * 1024>(src, off[3], at);
     if constexpr (LPS == 8) {
-      if (i == 4) ns_to_stage<4096>(src, off[4], at);
-      if (i == 5) ns_to_stage<5120>(src, off[5], at);
-      if (i == 6) ns_to_stage<6144>(src, off[6], at);
-      if (i == 7) ns_to_stage<7168>(src, off[7], at);
+      if (i == 4) ns_to_stage<4 * 1024>(src, off[4], at);
+      if (i == 5) ns_to_stage<5 * 1024>(src, off[5], at);
+      if (i == 6) ns_to_stage<6 * 1024>(src, off[6], at);
+      if (i == 7) ns_to_stage<7 * 1024>(src, off[7], at);
     }
     if (i == LPS - 1) src += step;
   };
@@ -568,7 +568,8 @@ enum { NS_NEXT = 0, NS_OUT = 1, NS_APPLY = 2 };
 
 // Eight consecutive values of the result, into the output or the parameters.
 template <int WHAT, typename O>
-__device__ __forceinline__ void ns_result(const NsArgs& p, const NsMat& m, int row, int col, const float* o, float keep, float rate) {
+__device__ __forceinline__ void ns_result(const NsArgs& p, const NsMat& m, int row, int col, const float* o, float keep,
+                                          float rate) {
   float v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = o[j];
@@ -915,7 +916,8 @@ __global__ __launch_bounds__(256) void ns_small_kernel(NsArgs p, int k) {
       if (WHAT == NS_NEXT)
         ns_small_put(tn, i, j + 2 * e, v);
       else
-        *(f32x4*)((float*)tn + i * NS_PITCH(64) + j + 2 * e) = f32x4{v[0] * unscale, v[1] * unscale, v[2] * unscale, v[3] * unscale};
+        *(f32x4*)((float*)tn + i * NS_PITCH(64) + j + 2 * e) =
+            f32x4{v[0] * unscale, v[1] * unscale, v[2] * unscale, v[3] * unscale};
     }
     __syncthreads();
     if (WHAT == NS_NEXT) {
@@ -929,7 +931,8 @@ __global__ __launch_bounds__(256) void ns_small_kernel(NsArgs p, int k) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int r = h * 32 + (threadIdx.x >> 3), c = (threadIdx.x & 7) * 8;
-        if (row0 + r < m.rows && col0 + c < m.cols) ns_result<WHAT, O>(p, m, row0 + r, col0 + c, (float*)tn + r * NS_PITCH(64) + c, keep, rate);
+        if (row0 + r < m.rows && col0 + c < m.cols)
+          ns_result<WHAT, O>(p, m, row0 + r, col0 + c, (float*)tn + r * NS_PITCH(64) + c, keep, rate);
       }
     }
     __syncthreads();

@@ -286,8 +286,8 @@ class NsPlan:
             ws = torch.empty(self.ws_elems, dtype=torch.float16, device=dev)
             part = torch.empty(self.parts + self.mats, dtype=torch.float64, device=dev)
             slabs = torch.empty(self.slabs * 4096, dtype=F32, device=dev) if self.slabs else None
-            args = NsArgs(*self.places, *self.counts, steps, DTYPES[inp.dtype], self.large, inp.data_ptr(), hipk.ptr(out), hipk.ptr(buf),
-                          hipk.ptr(w), hipk.ptr(w16), hipk.ptr(hyper), part.data_ptr(), hipk.ptr(slabs), ws.data_ptr(),
+            args = NsArgs(*self.places, *self.counts, steps, DTYPES[inp.dtype], self.large, inp.data_ptr(), hipk.ptr(out),
+                          hipk.ptr(buf), hipk.ptr(w), hipk.ptr(w16), hipk.ptr(hyper), part.data_ptr(), hipk.ptr(slabs), ws.data_ptr(),
                           self.parts, NORM_EPS, mu, wd, 1 if nesterov else 0)
             hipk.check(hipk.lib().dtfa_newton_schulz(C.byref(args), hipk.stream()), "newton_schulz")
 
