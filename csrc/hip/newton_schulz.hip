@@ -8,16 +8,23 @@
 // 0.68 .. 1.21.  Small singular values grow by a = 3.44 per iteration, and so does a rounding error made next to them:
 // with operands rounded to 16 bits the result is 1e-3 (well conditioned) to 1e-1 (low rank) off, with fp32 operands
 // 1e-6 to 2e-5.  There is no fp32 matrix instruction at more than a sixteenth of the fp16 rate, so the fp32 operands
-// are kept as two fp16 planes, hi + lo (22 bits), and a product is three v_mfma_f32_32x32x16_f16 --
-// hi*hi + hi*lo + lo*hi, the missing lo*lo is below 2^-22 of the sum of magnitudes -- into one fp32 accumulator.  fp16 and
-// not bf16 planes: the iterates are bounded (|f| <= 1.2024 on [0, 1.2024], so |X| <= 1.21, |A| <= 1.45, |B| <= 2.81 in every
-// entry), so a power of two per matrix puts them into fp16's range with 11 bits each instead of 8.
+// are kept as two fp16 planes, v = hi + 2^-11 lo (22 bits), and a product is three v_mfma_f32_32x32x16_f16: hi*hi into one
+// fp32 accumulator, hi*lo + lo*hi into another, 2^-11 of which is added at the end; the missing lo*lo is below 2^-22 of the
+// sum of magnitudes.  fp16 and not bf16 planes: the iterates are bounded (|f| <= 1.2024 on [0, 1.2024], so |X| <= 1.21, |A| <=
+// 1.45, |B| <= 2.81 in every entry), so a power of two puts them into fp16's range with 11 bits each instead of 8.
 //
-// Scales: X is held times S = 2^floor(log2(min(sqrt(rows * cols), 2^15))) -- entries of X_0 are at most 1 and of size
-// 1 / sqrt(rows * cols), later ones at most 1.21: nothing overflows 65504 and the lo plane's smallest step, 2^-24, is below
-// 2^-23 of a typical entry --, A and B times 2^14.  Where the norm is not far above eps, |X_0| = |G| / (|G| + eps) is small,
-// and grows by at most a < 4 per iteration: X_k is held times another 2^e_k, e_0 = -ceil(log2 |X_0|) found on the device
-// (with the norm), e_k = max(0, e_0 - 2 k), and A_k and B_k times 2^(2 e_k), so that vanishing gradients keep their bits.
+// Scales: X is held times S = 2^15, A and B times 2^14: nothing overflows 65504.  An entry that is small next to the others
+// grows by up to 3.44 per iteration relative to them, as much as its rounding error, so small entries need their bits as
+// well: a matrix with rows of 1e-6 is right only if these are.  That is why lo is held times 2^11, which keeps it in fp16's
+// normal range for as long as hi is: values of X keep 22 bits down to 2^-29 (of A and B to 2^-28) and are rounded to
+// multiples of 2^-50 below, where |X_0| is 1.  (With lo as it is, 2^-18 and 2^-40, and the scale going by the matrix's typical
+// entry: 128 x 256 with half of its rows times 1e-6 was 5e-4 of the norm off after 10 iterations, fp32 products 2e-6; in
+// rows of 1e-8 no bit was left.)  What is rounded away there grows to 3.44^12 2^-51 = 1e-9 of an entry in 12 iterations,
+// which is below what fp32 products lose; later ones would let it through.
+//
+// Where the norm is not far above eps, |X_0| = |G| / (|G| + eps) is small, and grows by at most a < 4 per iteration: X_k is
+// held times another 2^e_k, e_0 = -ceil(log2 |X_0|) found on the device (with the norm), e_k = max(0, e_0 - 2 k), and A_k
+// and B_k times 2^(2 e_k), so that vanishing gradients keep their bits.
 //
 // A and B are symmetric: only tiles on and below the diagonal are computed, their mirror images are copies.  All
 // matrices of an optimizer step (or of a batch) go through each stage in one launch, from work lists that name (matrix,
@@ -39,6 +46,7 @@ typedef f16 f16x4 __attribute__((ext_vector_type(4)));
 #define NS_B (-4.7750f)
 #define NS_C 2.0315f
 #define NS_GRAM_SCALE 16384.f  // of A and B
+#define NS_LO 2048.f           // of a lo plane against its hi plane
 
 // One matrix.  Offsets in elements of the buffer they point into.
 struct NsMat {
@@ -51,7 +59,7 @@ struct NsMat {
   int parts;
   int chunk;       // elements per partial sum
   int tall;        // rows > cols
-  float scale;     // S
+  float scale;     // S (the same for every matrix)
   float lr_scale;  // sqrt(max(1, rows / cols))
 };
 
@@ -145,8 +153,9 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs p) {
 
 __device__ __forceinline__ void ns_split(float v, f16& hi, f16& lo) {
   hi = (f16)v;
-  lo = (f16)(v - (float)hi);
+  lo = (f16)((v - (float)hi) * NS_LO);
 }
+__device__ __forceinline__ float ns_value(f16 hi, f16 lo) { return fmaf((float)lo, 1.f / NS_LO, (float)hi); }
 
 // A plane pair [rows][ld]: the hi value (row, col); its lo value is 32 further on.
 __device__ __forceinline__ size_t ns_at(int ld, int row, int col) {
@@ -156,7 +165,7 @@ __device__ __forceinline__ size_t ns_at(int ld, int row, int col) {
 __device__ __forceinline__ void ns_get(const f16* at, float (&v)[8]) {
   const f16x8 h = *(const f16x8*)at, l = *(const f16x8*)(at + 32);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = (float)h[j] + (float)l[j];
+  for (int j = 0; j < 8; ++j) v[j] = ns_value(h[j], l[j]);
 }
 __device__ __forceinline__ void ns_put(f16* at, const float (&v)[8]) {
   f16x8 h, l;
@@ -281,8 +290,7 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
   const int wr = wid >> 1, wc = wid & 1;
 
   // staging: this wave's half of an operand.  What stands beside the matrix instructions is kept short: the offsets of the
-  // lanes in registers, the k-tiles' start in scalar ones, places in LDS as constants of a loop over the slots (with all of
-  // it computed anew for every k-tile: 4096 x 4096 A 199, B 202, X 375 us instead of 187, 189 and 353).
+  // lanes in registers, the k-tiles' start in scalar ones, places in LDS moved by one addition each to the next slot.
   const bool kmajor = wid < 2 ? PK : QK;
   const int ld = wid < 2 ? P.ld : Q.ld, i0 = wid < 2 ? P.i0 : Q.i0;
   const f16* src = wid < 2 ? P.base : Q.base;
@@ -311,9 +319,9 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
   asm volatile("s_nop 4");
   const unsigned lds = (unsigned)(uintptr_t)(LDS_AS char*)smem;
   const unsigned lds_wave = lds + wid * (OPER / 2);
-  // (`i` and the slot are constants once the loops around are unrolled)
+  // (`i` is a constant once the loops around are unrolled; a slot is given by its first byte)
   auto stage_one = [&](int slot, int i) {
-    const unsigned at = lds_wave + slot * STAGE;
+    const unsigned at = lds_wave + slot;
     if (i == 0) ns_to_stage<0>(src, off[0], at);
     if (i == 1) ns_to_stage<1 * 1024>(src, off[1], at);
     if (i == 2) ns_to_stage<2 * 1024>(src, off[2], at);
@@ -347,25 +355,26 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
   unsigned p_at[2][2], q_at[2][2];
   places(PK, wr * (T / 2), 0, p_at);
   places(QK, wc * (T / 2), OPER, q_at);
-  auto frag = [&](bool km, const unsigned (&at)[2][2], int slot, int u, int ks, int lo) -> f16x8 {
+  auto frag = [&](bool km, const unsigned (&at)[2][2], int u, int ks, int lo) -> f16x8 {
     if (km) {
       union { s16x4 h[2]; f16x8 v; } r;
 #pragma unroll
       for (int q = 0; q < 2; ++q)
         r.h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (LDS_AS s16x4*)(uintptr_t)(at[lo][u] + slot * STAGE + (ks * 16 + 4 * q) * (T * 4)));
+            (LDS_AS s16x4*)(uintptr_t)(at[lo][u] + (ks * 16 + 4 * q) * (T * 4)));
       return r.v;
     }
-    return *(const LDS_AS f16x8*)(uintptr_t)(at[lo][ks] + slot * STAGE + u * 4096);
+    return *(const LDS_AS f16x8*)(uintptr_t)(at[lo][ks] + u * 4096);
   };
+  f32x16 cross[MT][MT];                       // sums of hi lo and lo hi, times NS_LO
   f16x8 ph[2][MT], pl[2][MT], qh[2][MT], ql[2][MT];
   constexpr int FRAGS = 4 * MT;               // of a step of 16 k: Q hi, P hi, Q lo, P lo
-  auto load_frag = [&](int slot, int ks, int to, int i) {
+  auto load_frag = [&](int ks, int to, int i) {
     const int u = i % MT;
-    if (i / MT == 0) qh[to][u] = frag(QK, q_at, slot, u, ks, 0);
-    if (i / MT == 1) ph[to][u] = frag(PK, p_at, slot, u, ks, 0);
-    if (i / MT == 2) ql[to][u] = frag(QK, q_at, slot, u, ks, 1);
-    if (i / MT == 3) pl[to][u] = frag(PK, p_at, slot, u, ks, 1);
+    if (i / MT == 0) qh[to][u] = frag(QK, q_at, u, ks, 0);
+    if (i / MT == 1) ph[to][u] = frag(PK, p_at, u, ks, 0);
+    if (i / MT == 2) ql[to][u] = frag(QK, q_at, u, ks, 1);
+    if (i / MT == 3) pl[to][u] = frag(PK, p_at, u, ks, 1);
   };
   // the matrix instructions of a step of 16 k; `between` issues other work behind each, which runs in its shadow
   auto multiply = [&](int from, auto between) {
@@ -374,7 +383,8 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
       const int u = n / MT % MT, v = n % MT;
       const f16x8 q = n / (MT * MT) == 1 ? ql[from][v] : qh[from][v];
       const f16x8 w = n / (MT * MT) == 2 ? pl[from][u] : ph[from][u];
-      acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q, w, acc[u][v], 0, 0, 0);
+      f32x16& to = n < MT * MT ? acc[u][v] : cross[u][v];
+      to = __builtin_amdgcn_mfma_f32_32x32x16_f16(q, w, to, 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
       between(n);
       __builtin_amdgcn_sched_barrier(0);
@@ -386,7 +396,7 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
 #pragma unroll
     for (int v = 0; v < MT; ++v)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[u][v][e] = 0.f;
+      for (int e = 0; e < 16; ++e) acc[u][v][e] = cross[u][v][e] = 0.f;
 
   const int nk = (k1 - k0) / NS_BK;
   auto stage = [&](int slot) {
@@ -395,7 +405,7 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
   };
 #pragma unroll
   for (int s = 0; s < NST - 1; ++s)
-    if (s < nk) stage(s);
+    if (s < nk) stage(s * STAGE);
   // waits until k-tile kt has arrived (the NST - 2 behind it may be on their way) and this wave's reads are done; after
   // the barrier that holds for every wave
   auto arrive = [&](int kt) {
@@ -405,48 +415,56 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
     asm volatile("" ::: "memory");
   };
   arrive(0);
-  if (NST - 1 < nk) stage(NST - 1);
+  if (NST - 1 < nk) stage((NST - 1) * STAGE);
 #pragma unroll
-  for (int i = 0; i < FRAGS; ++i) load_frag(0, 0, 0, i);
+  for (int i = 0; i < FRAGS; ++i) load_frag(0, 0, i);
   // Issued in a block, the eight LDS-DMA and eight LDS reads of a step would hold the wave for as long as its matrix
   // instructions take; one behind each of these they cost next to nothing.
   constexpr int N = 3 * MT * MT;
   constexpr int RPM = (FRAGS + N - 1) / N;    // reads, and LDS-DMA, behind one matrix instruction
   constexpr int SPM = (LPS + N - 1) / N;
-  auto second_half = [&](int slot) {
+  auto second_half = [&]() {
     multiply(0, [&](int n) {
 #pragma unroll
       for (int i = n * RPM; i < n * RPM + RPM; ++i)
-        if (i < FRAGS) load_frag(slot, 1, 1, i);
+        if (i < FRAGS) load_frag(1, 1, i);
     });
   };
   // (The last k-tile stands by itself: with one loop for all, the wait counts in front of the second group would have to
-  // hold for the pass without new reads as well, and wait for the new reads in all others.)
-  int last = -1;  // its slot
-  for (int kt = 0; last < 0; kt += NST) {
+  // hold for the pass without new reads as well, and wait for the new reads in all others.  The loop is not unrolled over
+  // the slots: the compiler would keep a second set of accumulators for its ways out.)
+  int slot = 0;
+  for (int kt = 0; kt + 1 < nk; ++kt) {
+    second_half();
+    arrive(kt + 1);  // ... and this k-tile has been read by every wave: its slot takes the one NST further on
+    const int here = slot;
+    slot = here == (NST - 1) * STAGE ? 0 : here + STAGE;
 #pragma unroll
-    for (int slot = 0; slot < NST; ++slot) {
-      const int nxt = (slot + 1) % NST;
-      if (kt + slot + 1 == nk) {
-        last = slot;
-        break;
+    for (int lo = 0; lo < 2; ++lo)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        p_at[lo][x] += slot - here;
+        q_at[lo][x] += slot - here;
       }
-      second_half(slot);
-      arrive(kt + slot + 1);  // ... and this k-tile has been read by every wave: its slot takes the one NST further on
-      const bool more = kt + slot + NST < nk;
-      multiply(1, [&](int n) {
+    const bool more = kt + NST < nk;
+    multiply(1, [&](int n) {
 #pragma unroll
-        for (int i = n * RPM; i < n * RPM + RPM; ++i)
-          if (i < FRAGS) load_frag(nxt, 0, 0, i);
-        if (more)
+      for (int i = n * RPM; i < n * RPM + RPM; ++i)
+        if (i < FRAGS) load_frag(0, 0, i);
+      if (more)
 #pragma unroll
-          for (int i = n * SPM; i < n * SPM + SPM; ++i)
-            if (i < LPS) stage_one(slot, i);
-      });
-    }
+        for (int i = n * SPM; i < n * SPM + SPM; ++i)
+          if (i < LPS) stage_one(here, i);
+    });
   }
-  second_half(last);
+  second_half();
   multiply(1, [](int) {});
+#pragma unroll
+  for (int u = 0; u < MT; ++u)
+#pragma unroll
+    for (int v = 0; v < MT; ++v)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[u][v][e] = fmaf(cross[u][v][e], 1.f / NS_LO, acc[u][v][e]);
 }
 
 // fp32 tile in LDS: 16-byte writes of 8 rows at a time hit every bank once at this pitch
@@ -693,6 +711,13 @@ __device__ __forceinline__ int ns_chunk(int row, int col, int lo) {
   return row * 256 + ((((col >> 5) * 8 + lo * 4 + ((col & 31) >> 3)) ^ ns_mix(row)) << 4);
 }
 
+__device__ __forceinline__ f32x16 ns_zero() {
+  f32x16 z;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) z[e] = 0.f;
+  return z;
+}
+
 // 64 x 64 product of two tiles over 64 k, added to `acc`; the wave's quarter, transposed as in ns_product
 template <bool PK, bool QK>
 __device__ __forceinline__ void ns_small_product(const char* P, const char* Q, f32x16& acc) {
@@ -712,14 +737,17 @@ __device__ __forceinline__ void ns_small_product(const char* P, const char* Q, f
     return *(const f16x8*)(tile + ns_chunk(row0 + (lane & 31), kk * 16 + (lane >> 5) * 8, lo));
   };
   const int i0 = (wid >> 1) * 32, j0 = (wid & 1) * 32;
+  f32x16 cross = ns_zero();
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk) {
     const f16x8 ph = frag(P, PK, i0, kk, 0), qh = frag(Q, QK, j0, kk, 0);
     const f16x8 pl = frag(P, PK, i0, kk, 1), ql = frag(Q, QK, j0, kk, 1);
     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, ph, acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql, ph, acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, pl, acc, 0, 0, 0);
+    cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql, ph, cross, 0, 0, 0);
+    cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, pl, cross, 0, 0, 0);
   }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = fmaf(cross[e], 1.f / NS_LO, acc[e]);
 }
 
 // four consecutive values of a tile, col a multiple of 4
@@ -727,7 +755,7 @@ __device__ __forceinline__ void ns_small_get(const char* tile, int row, int col,
   const int in = (col & 7) * 2;
   const f16x4 h = *(const f16x4*)(tile + ns_chunk(row, col, 0) + in), l = *(const f16x4*)(tile + ns_chunk(row, col, 1) + in);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = (float)h[j] + (float)l[j];
+  for (int j = 0; j < 4; ++j) v[j] = ns_value(h[j], l[j]);
 }
 __device__ __forceinline__ void ns_small_put(char* tile, int row, int col, const float (&v)[4]) {
   f16x4 h, l;
@@ -741,12 +769,6 @@ __device__ __forceinline__ void ns_small_put(char* tile, int row, int col, const
   const int in = (col & 7) * 2;
   *(f16x4*)(tile + ns_chunk(row, col, 0) + in) = h;
   *(f16x4*)(tile + ns_chunk(row, col, 1) + in) = l;
-}
-__device__ __forceinline__ f32x16 ns_zero() {
-  f32x16 z;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) z[e] = 0.f;
-  return z;
 }
 
 // a block of X: 64 rows of 256 bytes, `ld` elements apart per plane

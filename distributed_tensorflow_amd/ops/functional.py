@@ -1077,7 +1077,9 @@ def orthogonalize(x, steps: int = 5):
     """Every matrix ``x[..., :, :]`` with its singular values taken towards 1 by ``steps`` Newton-Schulz iterations
     ``X <- 3.4445 X - 4.7750 (X X^T) X + 2.0315 (X X^T)^2 X`` from ``x / (|x| + 1e-7)`` (Frobenius norm): what the Muon optimizer
     does to an update.  After five, singular values above about 1 % of the norm lie in 0.68 .. 1.21.  bf16, fp16 or fp32 on
-    the GPU, computed as accurately as in fp32 and rounded once; same shape and dtype, contiguous.  The matrices of a batch are
+    the GPU, computed as accurately as in fp32 in the norm of each matrix and rounded once; same shape and dtype, contiguous.
+    Entries down to 2^-29 of a matrix's norm keep their bits, smaller ones are rounded to multiples of 2^-50 of it: that
+    bounds ``steps``, each of which multiplies the smallest singular values by 3.44, to 12.  The matrices of a batch are
     independent, each normalised by itself; a zero matrix stays zero, one with an infinity or NaN becomes NaN as a
     whole.  Not differentiable."""
     if x.dim() < 2:

@@ -20,7 +20,8 @@ DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # as in row_i
 NORM_EPS = 1e-7
 MAX_SIDE = 1 << 20        # rows, columns
 MAX_SHORT_SIDE = 1 << 15  # the smaller of the two: its square is a plane of the workspace
-MAX_STEPS = 64
+MAX_STEPS = 12            # what the held bits of small entries carry (newton_schulz.hip)
+SCALE = 2.0 ** 15         # of X as it is held: entries of at most 1.21 stay below fp16's 65504
 MAX_PARTS = 1024          # partial sums of squares per matrix
 CHUNK = 8192              # elements per partial sum, at least
 
@@ -226,8 +227,7 @@ class NsPlan:
             n = rows * cols
             chunk = max(CHUNK, _up(-(-n // MAX_PARTS), CHUNK))
             parts = -(-n // chunk)
-            scale = 2.0 ** math.floor(math.log2(min(math.sqrt(n), 2.0 ** 15)))
-            mats[k] = (at, ws, ws + 4 * rp * cp, part, rows, cols, rp, cp, mp, parts, chunk, rows > cols, scale,
+            mats[k] = (at, ws, ws + 4 * rp * cp, part, rows, cols, rp, cp, mp, parts, chunk, rows > cols, SCALE,
                        math.sqrt(max(1.0, rows / cols)))
             ws += 4 * rp * cp + 4 * mp * mp
             part += parts
