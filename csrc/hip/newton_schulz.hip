@@ -23,8 +23,10 @@
 // which is below what fp32 products lose; later ones would let it through.
 //
 // Where the norm is not far above eps, |X_0| = |G| / (|G| + eps) is small, and grows by at most a < 4 per iteration: X_k is
-// held times another 2^e_k, e_0 = -ceil(log2 |X_0|) found on the device (with the norm), e_k = max(0, e_0 - 2 k), and A_k
-// and B_k times 2^(2 e_k), so that vanishing gradients keep their bits.
+// held times another 2^e_k, e_k = max(0, e_0 - 2 k), and A_k and B_k times 2^(2 e_k), so that vanishing gradients keep their
+// bits.  e_0 is found on the device (with the norm) so that 2^e_0 |X_0| is in [0.45, 0.9) or e_0 is 0: where c A A is scaled
+// away B_k is b A_k alone, up to 4.775 * 0.81 * 2^14 = 63370 (with 2^e_0 |X_0| up to 1 it overflowed 65504 on matrices in
+// which one row has nearly all of such a norm, and the result was NaN).
 //
 // A and B are symmetric: only tiles on and below the diagonal are computed, their mirror images are copies.  All
 // matrices of an optimizer step (or of a batch) go through each stage in one launch, from work lists that name (matrix,
@@ -191,7 +193,7 @@ __device__ __forceinline__ double ns_first_scale(const NsArgs& p, const NsMat& m
   const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3]));
   const double size = norm / (norm + (double)p.eps);
   lift = 0;
-  if (size > 0.0 && size < 1.0) (void)frexp(size, &lift);   // size * 2^-lift in [0.5, 1)
+  if (size > 0.0 && size < 1.0) (void)frexp(size / 0.9, &lift);   // size * 2^-lift in [0.45, 0.9)
   lift = lift < 0 ? -lift : 0;
   return ldexp((double)m.scale / (norm + (double)p.eps), lift);
 }
