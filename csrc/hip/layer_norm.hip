@@ -469,24 +469,29 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_few_kernel(LnBwd p, unsign
 }
 
 // [parts][2][cols] -> dgamma, dbeta.  32 columns x 32 row lanes: lane r sums parts r, r + 32, ... and the lanes are
-// added in order, so the result does not depend on scheduling.
+// added in order, so the result does not depend on scheduling.  Workgroups walk over the columns: one each would be more
+// than the 2^32 threads of a launch from 2^26 columns on.
 __global__ __launch_bounds__(1024) void layer_norm_params_kernel(const float* __restrict__ part, int parts, int cols,
                                                                  float* __restrict__ dgamma, float* __restrict__ dbeta) {
   __shared__ float red[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const long long e = (long long)blockIdx.x * 32 + tx, n = 2LL * cols;
-  float s = 0.f;
-  if (e < n)
+  const long long n = 2LL * cols;
+  for (long long e0 = (long long)blockIdx.x * 32; e0 < n; e0 += (long long)gridDim.x * 32) {
+    const long long e = e0 + tx;
+    float s = 0.f;
+    if (e < n)
 #pragma unroll 8
-    for (int k = ty; k < parts; k += 32) s += part[(size_t)k * n + e];
-  red[ty][tx] = s;
-  __syncthreads();
-  if (ty == 0 && e < n) {
-    float t = 0.f;
+      for (int k = ty; k < parts; k += 32) s += part[(size_t)k * n + e];
+    red[ty][tx] = s;
+    __syncthreads();
+    if (ty == 0 && e < n) {
+      float t = 0.f;
 #pragma unroll
-    for (int r = 0; r < 32; ++r) t += red[r][tx];
-    float* out = e < cols ? dgamma : dbeta;
-    if (out != nullptr) out[e < cols ? e : e - cols] = t;
+      for (int r = 0; r < 32; ++r) t += red[r][tx];
+      float* out = e < cols ? dgamma : dbeta;
+      if (out != nullptr) out[e < cols ? e : e - cols] = t;
+    }
+    __syncthreads();
   }
 }
 
@@ -741,7 +746,8 @@ extern "C" int dtfa_layer_norm_bwd(const void* x, long long ldx, const void* dy,
            : dtype == IO_F16 ? ln_bwd<f16>(p, nvec, grid, dgamma, dbeta, st)
            : dtype == IO_F32 ? ln_bwd<float>(p, nvec, grid, dgamma, dbeta, st) : -2;
   if (rc != 0 || part == nullptr) return rc;
-  hipLaunchKernelGGL(layer_norm_params_kernel, dim3((unsigned)((2LL * cols + 31) / 32)), dim3(1024), 0, st, part, parts,
-                     cols, dgamma, dbeta);
+  const long long strips = (2LL * cols + 31) / 32;
+  hipLaunchKernelGGL(layer_norm_params_kernel, dim3((unsigned)(strips < LN_MAX_GRID ? strips : LN_MAX_GRID)), dim3(1024), 0, st,
+                     part, parts, cols, dgamma, dbeta);
   return (int)hipGetLastError();
 }
