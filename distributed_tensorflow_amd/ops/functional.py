@@ -25,7 +25,7 @@ import os
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import conv as cv
@@ -57,6 +57,13 @@ def _use_hip(t: torch.Tensor) -> bool:
 
 def _needs_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _is_dual(*tensors) -> bool:
+    """Whether a tensor carries a tangent of forward-mode differentiation: it does not require grad, and a kernel that reads
+    its memory would lose the tangent."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                                  for t in tensors)
 
 
 def concat_plan(x: torch.Tensor, *tensors) -> bool:
@@ -1056,7 +1063,8 @@ def layer_norm(x, gamma=None, beta=None, eps: float = 1e-5):
     """Normalise every vector along the last axis of ``x`` to mean 0 and variance 1 (biased, ``eps`` added to it), then
     scale by ``gamma`` and shift by ``beta`` (vectors, either may be None).  On the GPU ``x`` is bf16, fp16 or fp32 --
     contiguous or a channel slice of a wider tensor; other layouts are copied first --, ``gamma`` / ``beta`` are fp32, and
-    the result is contiguous in ``x``'s dtype.  Differentiable once in all three.  (As with every operator, a backward pass
+    the result is contiguous in ``x``'s dtype.  Differentiable once in all three, backwards (forward-mode tangents are refused
+    on the GPU).  (As with every operator, a backward pass
     over leaves can be captured into a graph only while no eager graph over the same leaves is alive.)"""
     if not _use_hip(x):
         if x.dim() < 1 or x.shape[-1] < 1:
@@ -1065,6 +1073,8 @@ def layer_norm(x, gamma=None, beta=None, eps: float = 1e-5):
             if t is not None and tuple(t.shape) != (x.shape[-1],):
                 raise ValueError("layer_norm: %s must be a vector of %d elements, got %s" % (nm, x.shape[-1], tuple(t.shape)))
         return ref.layer_norm(x, gamma, beta, eps)
+    if _is_dual(x, gamma, beta):
+        raise ValueError("layer_norm has no forward-mode derivative on the GPU")
     if not _needs_grad(x, gamma, beta):
         return K.layer_norm_fwd(x, gamma, beta, eps)[0]
     return _LayerNormFn.apply(x, gamma, beta, eps, (gamma, beta))
@@ -1089,7 +1099,7 @@ def orthogonalize(x, steps: int = 5):
     if not x.dtype.is_floating_point:
         raise ValueError("orthogonalize: x must be of a floating-point type, got %s" % x.dtype)
     ns.check_shape(x.shape[-2], x.shape[-1], "orthogonalize")
-    if _needs_grad(x):
+    if _needs_grad(x) or _is_dual(x):
         raise ValueError("orthogonalize is not differentiable: call it under torch.no_grad() or on x.detach()")
     if not _use_hip(x):
         return ref.newton_schulz(x, steps)
