@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from collections import Counter
 from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -24,6 +25,9 @@ MAX_STEPS = 12            # what the held bits of small entries carry (newton_sc
 SCALE = 2.0 ** 15         # of X as it is held: entries of at most 1.21 stay below fp16's 65504
 MAX_PARTS = 1024          # partial sums of squares per matrix
 CHUNK = 8192              # elements per partial sum, at least
+# Workspace of a batch: larger ones go in groups, one after the other (a matrix at least).  A group fills the card many times
+# over: with 256 MiB 64 of 1024 x 1024 took 5.66 instead of 5.29 ms, 40 of 64 x 8192 0.52 instead of 0.43.
+GROUP_BYTES = 2 << 30
 
 # Measured on one MI355X, a CU's time in us: a tile job's fixed part (its first loads, the epilogue) and a k-step of 32.
 # A 128 x 128 tile does four times the work of a 64 x 64 tile in twice the time, so large tiles win once there are enough
@@ -114,14 +118,15 @@ def _choose(dims: Sequence[Tuple[int, int, int]], symmetric: bool) -> Tuple[int,
     """(size of the shorter of tile rows / columns from which tiles are 128, longest piece of a reduction in k-steps) of a
     stage whose outputs are ``rows x cols`` sums over ``K`` for (rows, cols, K) in ``dims``."""
     best: Optional[Tuple[float, int, int]] = None
+    alike = Counter(dims)
     for large_from in (128, 256, 512, 1024, 1 << 30):
         for piece in (1 << 30, 64, 48, 40, 32, 28, 24, 20, 16, 12, MIN_STEPS) if symmetric else (1 << 30,):
             jobs: Dict[float, int] = {}
             slabs = 0
-            for rows, cols, K in dims:
+            for (rows, cols, K), many in alike.items():
                 edge = 128 if min(rows, cols) >= large_from else 64
                 tr, tc, steps = -(-rows // edge), -(-cols // edge), _up(K, edge) // 32
-                n = tr * (tr + 1) // 2 if symmetric else tr * tc
+                n = (tr * (tr + 1) // 2 if symmetric else tr * tc) * many
                 cut = -(-steps // piece)
                 cost = _job_us(edge, -(-steps // cut))
                 jobs[cost] = jobs.get(cost, 0) + n * cut
@@ -168,6 +173,17 @@ def _cut_tail(jobs: np.ndarray, slabs: int) -> Tuple[np.ndarray, np.ndarray, int
     piece = max(MIN_STEPS, -(-steps // max(2, SLOTS // tail)))
     cut, joins, slabs = _cut(jobs[-tail:], piece, slabs)
     return np.concatenate([jobs[:-tail], cut]), joins, slabs
+
+
+def _repeat(jobs: np.ndarray, n: int, mat: int, slab: int = 0, slabs: int = 0) -> np.ndarray:
+    """The jobs of one matrix for ``n`` alike from number ``mat`` on, whose slabs follow one another from ``slab`` on,
+    ``slabs`` for each."""
+    out = np.tile(jobs, (n, 1))
+    which = np.repeat(np.arange(n, dtype=np.int32), len(jobs))
+    out[:, 0] = mat + which
+    if jobs.shape[1] == 8:
+        out[:, 6] = np.where(out[:, 6] >= 0, out[:, 6] + slab + which * slabs, out[:, 6])
+    return out
 
 
 def _join(parts: Sequence[np.ndarray], width: int = 8) -> np.ndarray:
@@ -220,45 +236,62 @@ class NsPlan:
         chunks, packs, gram, gram_joins, poly, poly_joins, full = [], [], [], [], [], [], []
         small: List[np.ndarray] = []
         ws = part = gram_slabs = poly_slabs = small_slices = 0
-        for k, (at, rows, cols) in enumerate(matrices):
+        k = 0
+        while k < len(matrices):   # runs of matrices of one shape
+            _, rows, cols = matrices[k]
+            many = 1
+            while k + many < len(matrices) and tuple(matrices[k + many][1:]) == (rows, cols):
+                many += 1
             short = min(rows, cols)
             edge = 128 if short >= min(gram_large, poly_large, full_large) else 64
             rp, cp, mp = _up(rows, edge), _up(cols, edge), _up(short, edge)
             n = rows * cols
             chunk = max(CHUNK, _up(-(-n // MAX_PARTS), CHUNK))
             parts = -(-n // chunk)
-            mats[k] = (at, ws, ws + 4 * rp * cp, part, rows, cols, rp, cp, mp, parts, chunk, rows > cols, SCALE,
-                       math.sqrt(max(1.0, rows / cols)))
-            ws += 4 * rp * cp + 4 * mp * mp
-            part += parts
+            elems = 4 * rp * cp + 4 * mp * mp
+            run = mats[k:k + many]
+            run["at"] = [at for at, _, _ in matrices[k:k + many]]
+            run["x"] = ws + np.arange(many, dtype=np.int64) * elems
+            run["a"] = run["x"] + 4 * rp * cp
+            run["part"] = part + np.arange(many, dtype=np.int64) * parts
+            for name, v in (("rows", rows), ("cols", cols), ("rp", rp), ("cp", cp), ("mp", mp), ("parts", parts),
+                            ("chunk", chunk), ("tall", rows > cols), ("scale", SCALE),
+                            ("lr_scale", math.sqrt(max(1.0, rows / cols)))):
+                run[name] = v
+            ws += many * elems
+            part += many * parts
+            i = np.arange(parts, dtype=np.int32)
+            chunks.append(_repeat(np.stack([0 * i, i, 0 * i, 0 * i], 1), many, k))
             if fused:
                 blocks = max(rp, cp) // 64
                 slices = min(blocks, max(1, round(math.sqrt(SMALL_BLOCKS_PER_SLICE2 * blocks))))
                 edges = np.arange(slices + 1) * blocks // slices
-                jobs = _jobs(k, np.arange(slices), edges[:-1], np.diff(edges), slices, 0, small_slices)
-                small.append(jobs)
-                small_slices += slices
-            chunks.append(np.stack([np.full(parts, k), np.arange(parts), np.zeros(parts), np.zeros(parts)], 1).astype(np.int32))
+                jobs = _jobs(0, np.arange(slices), edges[:-1], np.diff(edges), slices, 0, 0)
+                small.append(_repeat(jobs, many, k, small_slices, slices))
+                small_slices += many * slices
+                k += many
+                continue
             i, j = _tiles(rp // 64, cp // 64)
-            packs.append(np.stack([np.full_like(i, k), i, j, np.zeros_like(i)], 1).astype(np.int32))
+            packs.append(_repeat(np.stack([0 * i, i, j, 0 * i], 1).astype(np.int32), many, k))
             e = 128 if short >= gram_large else 64
-            tiles = _jobs(k, *_tiles(mp // e, mp // e, lower=True), e, 0, max(rp, cp))
-            jobs, joins, gram_slabs = _cut(tiles, gram_piece, gram_slabs)
+            jobs, joins, used = _cut(_jobs(0, *_tiles(mp // e, mp // e, lower=True), e, 0, max(rp, cp)), gram_piece, 0)
             if len(matrices) == 1 and not len(joins):
-                jobs, joins, gram_slabs = _cut_tail(jobs, gram_slabs)
-            gram.append(jobs)
-            gram_joins.append(joins)
+                jobs, joins, used = _cut_tail(jobs, 0)
+            gram += np.split(_repeat(jobs, many, k, gram_slabs, used), many)
+            gram_joins.append(_repeat(joins, many, k, gram_slabs, used))
+            gram_slabs += many * used
             e = 128 if short >= poly_large else 64
-            jobs, joins, poly_slabs = _cut(_jobs(k, *_tiles(mp // e, mp // e, lower=True), e, 0, mp), poly_piece, poly_slabs)
+            jobs, joins, used = _cut(_jobs(0, *_tiles(mp // e, mp // e, lower=True), e, 0, mp), poly_piece, 0)
             if len(matrices) == 1 and not len(joins):
-                jobs, joins, poly_slabs = _cut_tail(jobs, poly_slabs)
-            poly.append(jobs)
-            poly_joins.append(joins)
+                jobs, joins, used = _cut_tail(jobs, 0)
+            poly += np.split(_repeat(jobs, many, k, poly_slabs, used), many)
+            poly_joins.append(_repeat(joins, many, k, poly_slabs, used))
+            poly_slabs += many * used
             e = 128 if short >= full_large else 64
-            full.append(_jobs(k, *_tiles(rp // e, cp // e), e, 0, mp))
-        if fused:   # one launch an iteration, no other jobs
-            packs, gram, gram_joins, poly, poly_joins, full = [], [], [], [], [], []
-            gram_slabs, poly_slabs = 2 * small_slices, 0
+            full += np.split(_repeat(_jobs(0, *_tiles(rp // e, cp // e), e, 0, mp), many, k), many)
+            k += many
+        if fused:   # one launch an iteration
+            gram_slabs = 2 * small_slices
         slabs = max(gram_slabs, poly_slabs)   # (a stage's slabs are joined before the next stage writes its own)
         lists = [np.concatenate(chunks), _join(packs, 4), _over_xcds(gram), _join(gram_joins), _over_xcds(poly),
                  _join(poly_joins), _over_xcds(full), _join(small)]
@@ -307,6 +340,15 @@ def get_plan(key: tuple, matrices: Callable[[], Sequence[Tuple[int, int, int]]],
     return plan
 
 
+def _group(rows: int, cols: int) -> int:
+    """How many matrices of a batch go together at most: what GROUP_BYTES hold of their planes, padded to tiles, and slabs."""
+    short, long = sorted((rows, cols))
+    edge = 64 if short <= 64 else 128
+    m, n = _up(short, edge), _up(long, edge)
+    slabs = 2 * (n // 64) * 4096 * 4 if short <= 64 else m * m * 4
+    return max(1, GROUP_BYTES // (8 * (m * n + m * m) + slabs))
+
+
 def orthogonalize(x: torch.Tensor, steps: int) -> torch.Tensor:
     """``x [..., rows, cols]`` on the GPU -> the same shape and dtype (bf16, fp16 or fp32), contiguous."""
     if not x.is_cuda:
@@ -318,9 +360,15 @@ def orthogonalize(x: torch.Tensor, steps: int) -> torch.Tensor:
     out = torch.empty_like(x)
     if x.numel() == 0:
         return out
-    batch = x.numel() // (rows * cols)
-    plan = get_plan((batch, rows, cols), lambda: [(i * rows * cols, rows, cols) for i in range(batch)], x.device)
-    plan.launch(inp=x, steps=steps, out=out)
+    n = rows * cols
+    batch = x.numel() // n
+    groups = -(-batch // _group(rows, cols))
+    for k in range(groups):
+        first = k * batch // groups
+        many = (k + 1) * batch // groups - first
+        plan = get_plan((many, rows, cols), lambda: [(i * n, rows, cols) for i in range(many)], x.device)
+        part = slice(first * n, (first + many) * n)
+        plan.launch(inp=x.view(-1)[part], steps=steps, out=out.view(-1)[part])
     return out
 
 
