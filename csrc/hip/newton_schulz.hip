@@ -859,7 +859,7 @@ __global__ __launch_bounds__(256) void ns_small_first_kernel(NsArgs p) {
 
 // Iteration k of a slice; the partial products of iteration k are in half k % 2 of the slabs.
 template <int WHAT, typename O, bool SHIFT>
-__global__ __launch_bounds__(256) void ns_small_kernel(NsArgs p, int k) {
+__global__ __launch_bounds__(256, 3) void ns_small_kernel(NsArgs p, int k) {
   __shared__ __attribute__((aligned(16))) char lds[2 * NS_TILE + 64 * NS_PITCH(64) * 4];
   __shared__ f32x4 diagonal[4];  // every fourth value of A's
   char* tb = lds;                 // F
