@@ -143,6 +143,12 @@ class Saver:
                 m[id(seg.param)] = (g.name, seg.offset, seg.numel)
         return m
 
+    def _slot_covers(self, key: str, offset: int) -> bool:
+        """Whether the parameter at ``offset`` of its flat buffer has the slot ``key`` (Muon's kernels have no Adam moments)."""
+        optimizer = getattr(self.engine, "optimizer", None)
+        spans = optimizer.slot_spans().get(key) if hasattr(optimizer, "slot_spans") else None
+        return spans is None or any(at <= offset < at + n for at, n in spans)
+
     def variables(self, include_slots: bool = True, detach_host: bool = False) -> Dict[str, np.ndarray]:
         """TensorFlow-named arrays of every variable.  ``detach_host``: arrays never alias live host tensors
         (what a background writer needs while training keeps updating them)."""
@@ -180,7 +186,7 @@ class Saver:
             if loc is not None:
                 for key, flat in slots.items():
                     slot, g2 = key.rsplit("/", 1)
-                    if g2 != gname:
+                    if g2 != gname or not self._slot_covers(key, off):
                         continue
                     sv = flat[off:off + n].view(t.shape)
                     out[spec.name + "/" + SLOT_SUFFIX.get(slot, slot)] = host(spec.to_tf(sv.float()))
@@ -271,7 +277,7 @@ class Saver:
                 for key, flat in slots.items():
                     slot, g2 = key.rsplit("/", 1)
                     name = spec.name + "/" + SLOT_SUFFIX.get(slot, slot)
-                    if g2 == gname and name in data:
+                    if g2 == gname and name in data and self._slot_covers(key, off):
                         sv = spec.from_tf(torch.from_numpy(np.asarray(data[name], dtype=np.float32)),
                                           t.detach().float().cpu())
                         if key not in new_slots:

@@ -125,6 +125,10 @@ class _RegionOptimizer:
     def slots(self) -> Dict[str, torch.Tensor]:
         raise NotImplementedError
 
+    def slot_spans(self) -> Dict[str, Sequence[Tuple[int, int]]]:
+        """(offset, length) of the values that a slot belongs to, for slots that do not belong to their whole region."""
+        return {}
+
 
 class FusedAdam(_RegionOptimizer):
     def __init__(self, regions: List[OptRegion], lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8):
@@ -328,6 +332,13 @@ class FusedMuon(_RegionOptimizer):
         out = {"Momentum/" + k: t for k, t in self.buf.items()}
         out.update({"Adam/" + k: t for k, t in self.m.items()})
         out.update({"Adam_1/" + k: t for k, t in self.v.items()})
+        return out
+
+    def slot_spans(self):
+        out = {}
+        for r in self.regions:
+            out["Momentum/" + r.name] = [(at, rows * cols) for at, rows, cols in r.matrices]
+            out["Adam/" + r.name] = out["Adam_1/" + r.name] = list(r.vectors)
         return out
 
 
