@@ -1069,6 +1069,8 @@ def layer_norm(x, gamma=None, beta=None, eps: float = 1e-5):
     if not _use_hip(x):
         if x.dim() < 1 or x.shape[-1] < 1:
             raise ValueError("layer_norm: the last axis must not be empty, got shape %s" % (tuple(x.shape),))
+        if not x.dtype.is_floating_point:
+            raise ValueError("layer_norm: x must be of a floating-point type, got %s" % x.dtype)
         for t, nm in ((gamma, "gamma"), (beta, "beta")):
             if t is not None and tuple(t.shape) != (x.shape[-1],):
                 raise ValueError("layer_norm: %s must be a vector of %d elements, got %s" % (nm, x.shape[-1], tuple(t.shape)))
