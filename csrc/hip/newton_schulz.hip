@@ -34,11 +34,15 @@
 // tiles, so the products need no bounds checks; a row holds its two planes in turns of 32 values, hi then lo, so that the
 // 32 k of a step are one 128-byte line per row (apart, each plane's 64 bytes fetched a line of which half was used).
 //
-// Measured: 4096 x 4096, an iteration A 187 us, B 189 us, X 353 us: 1.1 .. 1.2 PFLOP/s in the matrix cores, next to 1.45
-// of the fastest large fp16 product on this card.  ResNet-50's 54 matrices, an iteration A 57 + 12, B 29, X 105 us: X's
+// Measured: 4096 x 4096, an iteration A 191 us, B 194 us, X 346 us: 1.1 .. 1.2 PFLOP/s in the matrix cores, next to 1.45
+// of the fastest large fp16 product on this card.  ResNet-50's 54 matrices, an iteration A 61 + 12, B 32, X 108 us: X's
 // tiles have as few as two k-steps, so that what they take is their first loads and the 128 KB of X that each reads and
-// writes at its end; norm and first iterate 56 and 65 us at 5 TB/s, the last X with the parameters 132.  Up to a few hundred
+// writes at its end; norm and first iterate 56 and 65 us at 5 TB/s, the last X with the parameters 140.  Up to a few hundred
 // rows an iteration is four launches of 4 .. 15 us, 5 of them a tile's first loads and its end.
+//
+// Errors of fp32 results after five iterations are 0.2 .. 0.6 times those of fp32 with sums by blocks on sides of up to 64 and
+// 0.6 .. 1.25 times on longer ones (0.3 .. 0.6 times those of the fp32 library products from 2500 on), single matrices of
+// a few entries up to 2.5 times; after twelve up to twice.
 #include "row_io.h"
 
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
@@ -277,9 +281,14 @@ __device__ __forceinline__ void ns_to_stage(const f16* base, unsigned off, unsig
 //
 // What bounds it is LDS: a k-tile of 128 x 128 is 32 KB written and 64 KB read, 768 cycles at 128 bytes a cycle, next to
 // 768 cycles of matrix instructions on each of the four SIMDs; one of 64 x 64 is 48 KB, 384 cycles, next to 192.  NST is 2
-// for 128 x 128.  64 x 64 tiles have three slots, so that three workgroups fit a CU, but A and B four where they are at most
-// two to a CU (36 tiles over 8192 values: 59 -> 46 us, with six no less; 872 tiles over up to 1024: 29.9 us with three slots,
-// 32.4 with four; 531 of X: 12.3 and 13.3).
+// for 128 x 128.  64 x 64 tiles of A and B have four slots where they are at most two to a CU, which is what their registers
+// (213) leave room for (36 tiles over 8192 values: 59 -> 46 us, with six no less), else three: ResNet-50's update, whose B
+// has 872 tiles over up to 1024 values, 1148 us with three there and 1159 with four.
+//
+// The sums of hi hi and of the mixed products have accumulators of their own, so that lo may have a scale of its own.  It
+// also makes for two thirds fewer roundings in the large sums: 4096 x 4096 fp32 1.7e-6 of the norm off, in one accumulator
+// 3.2e-6.  For 128 x 128 that is 128 registers of accumulators next to 64 of fragments: the loop over k-tiles must be a
+// single body with one way out, or the compiler holds accumulators twice and spills.
 template <int T, int NST, bool PK, bool QK>
 __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& Q, int k0, int k1, char* smem,
                                            f32x16 (&acc)[T / 64][T / 64]) {
@@ -471,7 +480,7 @@ __device__ __forceinline__ void ns_product(const NsOperand& P, const NsOperand& 
 
 // fp32 tile in LDS: 16-byte writes of 8 rows at a time hit every bank once at this pitch
 #define NS_PITCH(T) ((T) + 4)
-// LDS of a launch with large tiles or four slots (two workgroups to a CU), and of others (three)
+// LDS of a launch with large tiles or four slots (two workgroups to a CU), and of others
 #define NS_LDS_LARGE (128 * NS_PITCH(128) * 4)
 #define NS_LDS_SMALL (3 * 4 * 64 * NS_BK * 2)
 static_assert(NS_LDS_LARGE >= 2 * 4 * 128 * NS_BK * 2 && NS_LDS_LARGE >= 4 * 4 * 64 * NS_BK * 2, "stages fit");
@@ -701,8 +710,9 @@ __global__ __launch_bounds__(256, 2) void ns_advance_kernel(NsArgs p, int k) {
 // algebra holds for any d, but all workgroups of a matrix must take the same), and
 //   B = (b d + c d^2) I + F,   F = (b + 2 c d) E + c E E,   X_{k+1} = (a + b d + c d^2) X_k + F X_k:
 // E and F are small where A is close to the identity, and so is all that their products and their 22 bits lose (12 x 500:
-// 2.0e-6 of the norm off with d = 0, 0.6e-6 with this, 1.6e-6 in fp32 products).  It takes 0.5 us an iteration, so results
-// that are rounded to 16 bits, and updates of parameters, which they reach times a small rate, are made with d = 0.
+// 7.4e-7 of the norm off with d = 0, 2.4e-7 with this, 7.9e-7 in fp32 products).  It takes 0.5 us an iteration, so results
+// that are rounded to 16 bits, and updates of parameters, which they reach times a small rate, are made with d = 0: 0.3 .. 1.3
+// times the error of fp32 products.
 //
 // Tiles in LDS: 64 rows of 256 bytes, two blocks of 32 columns, hi and lo.  One swizzle serves both ways of reading:
 // 16 rows at one chunk (all four bits of the row differ) and 64 bytes in four consecutive rows (its low bits on top).

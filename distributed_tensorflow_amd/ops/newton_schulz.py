@@ -37,7 +37,7 @@ STEP_US = {128: 0.72, 64: 0.31}
 JOIN_US, JOIN_US_PER_BYTE = 4.0, 0.25e-6   # the launch that joins cut reductions (8 MB of slabs 6 us, 127 MB 36 us)
 CUS = 256
 SLOTS = 2 * CUS           # workgroups at a time
-MIN_STEPS = 8             # shortest piece of a cut reduction
+MIN_STEPS = 8             # least upper bound of the pieces of a cut reduction (cut evenly: 9 k-steps make pieces of 4 and 5)
 
 # Shorter sides of at most 64 take one launch an iteration, in which every workgroup adds up the partial products of all
 # slices of its matrix (about 0.25 us each) and advances the 64 x 64 blocks of its own (about 2.5 us each): the time is
